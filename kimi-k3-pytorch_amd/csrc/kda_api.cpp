@@ -635,4 +635,85 @@ int kda_layer_decode(const kda_layer_decode_args* args, void* stream) {
   return launch_layer_decode(d, static_cast<hipStream_t>(stream));
 }
 
+static int check_norm(const char* what, const void* in, int64_t rows, int64_t width, double eps, int dtype,
+                      bool f64_allowed) {
+  g_detail[0] = '\0';
+  if (!is_input_dtype(dtype) || (dtype == KDA_DTYPE_F64 && !f64_allowed)) {
+    set_detail("%s: bad dtype %d", what, dtype);
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  if (rows <= 0 || width <= 0 || rows > INT64_MAX / 8 / width) {
+    set_detail("%s: sizes must be positive (rows=%lld width=%lld)", what, (long long)rows, (long long)width);
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  if (!in) {
+    set_detail("%s: the input must be non-null", what);
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  if (!(eps > 0.0)) {
+    set_detail("%s: eps must be > 0", what);
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  return KDA_OK;
+}
+
+int kda_add_rmsnorm_fwd(const void* x, const void* residual, const void* weight, void* h, void* y, int64_t rows,
+                        int64_t width, double eps, int dtype, void* stream) {
+  const int rc = check_norm("add_rmsnorm", x, rows, width, eps, dtype, true);
+  if (rc != KDA_OK) return rc;
+  if (!y || (residual && !h)) {
+    set_detail("add_rmsnorm: y (and h with a residual) must be non-null");
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  return launch_add_norm(x, residual, weight, h, y, nullptr, nullptr, width, rows, width, eps, dtype,
+                         static_cast<hipStream_t>(stream));
+}
+
+int kda_add_rmsnorm_quant(const void* x, const void* residual, const void* weight, void* h, void* q, float* scales,
+                          int64_t group, int64_t rows, int64_t width, double eps, int dtype, void* stream) {
+  const int rc = check_norm("add_rmsnorm_quant", x, rows, width, eps, dtype, false);
+  if (rc != KDA_OK) return rc;
+  if (!q || !scales || (residual && !h)) {
+    set_detail("add_rmsnorm_quant: q, scales (and h with a residual) must be non-null");
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  const bool listed = group == 32 || group == 64 || group == 128 || group == 256;
+  if (group != width && (!listed || width % group != 0)) {
+    set_detail("add_rmsnorm_quant: groups of 32, 64, 128 or 256 that divide the width %lld, or the width, got %lld",
+               (long long)width, (long long)group);
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  return launch_add_norm(x, residual, weight, h, nullptr, q, scales, group, rows, width, eps, dtype,
+                         static_cast<hipStream_t>(stream));
+}
+
+size_t kda_add_rmsnorm_bwd_workspace_bytes(int64_t rows, int64_t width, int dtype) {
+  if (rows <= 0 || width <= 0 || !is_input_dtype(dtype)) return 0;
+  return add_norm_bwd_workspace_bytes(rows, width, dtype);
+}
+
+int kda_add_rmsnorm_bwd(const void* h, const void* weight, const void* d_y, const void* d_h, void* dx, void* d_weight,
+                        int64_t rows, int64_t width, double eps, int dtype, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  const int rc = check_norm("add_rmsnorm_bwd", h, rows, width, eps, dtype, true);
+  if (rc != KDA_OK) return rc;
+  if (!d_y || !dx) {
+    set_detail("add_rmsnorm_bwd: d_y and dx must be non-null");
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  if (d_weight) {
+    const size_t need = add_norm_bwd_workspace_bytes(rows, width, dtype);
+    if (!workspace || workspace_bytes < need) {
+      set_detail("add_rmsnorm_bwd: workspace of %zu bytes needed", need);
+      return KDA_ERR_WORKSPACE;
+    }
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) {
+      set_detail("add_rmsnorm_bwd: the workspace must be 16-byte aligned");
+      return KDA_ERR_INVALID_ARGUMENT;
+    }
+  }
+  return launch_add_norm_bwd(h, weight, d_y, d_h, dx, d_weight, rows, width, eps, dtype, workspace,
+                             static_cast<hipStream_t>(stream));
+}
+
 }  // extern "C"

@@ -112,6 +112,10 @@ SIGNATURES = {
     "kda_mask_lengths": (_I, [_P, _L, _L, _P, _P]),
     "kda_layer_decode_workspace_bytes": (_S, [_P]),
     "kda_layer_decode": (_I, [_P, _P]),
+    "kda_add_rmsnorm_fwd": (_I, [_P] * 5 + [_L, _L, ctypes.c_double, _I, _P]),
+    "kda_add_rmsnorm_quant": (_I, [_P] * 6 + [_L, _L, _L, ctypes.c_double, _I, _P]),
+    "kda_add_rmsnorm_bwd_workspace_bytes": (_S, [_L, _L, _I]),
+    "kda_add_rmsnorm_bwd": (_I, [_P] * 6 + [_L, _L, ctypes.c_double, _I, _P, _S, _P]),
 }
 
 _lock = threading.Lock()

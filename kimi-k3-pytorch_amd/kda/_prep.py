@@ -91,3 +91,24 @@ def longest_document(offsets: list[int] | None) -> int:
 
 def stream(device: torch.device) -> int:
     return _lib.stream_of(device)
+
+
+class _Here:
+    """The current device is the tensors' own: nothing to switch."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return None
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """The tensors' GPU as the current one for a launch: a kernel and its
+    stream have to be of one device.  Free where it is so already."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)

@@ -14,6 +14,8 @@
 * ``rmsnorm_gate``: HeadwiseRMSNorm (src/kimi_primitives/headwise_rmsnorm.py:39-64)
   times the sigmoid output gate (src/kimi_primitives/output_gate.py:62-75),
   i.e. the input of the output projection.
+* ``add_rmsnorm``: the RMSNorm that enters a layer, with the residual's
+  addition; ``add_rmsnorm_quant`` gives it in 8 bits (e4m3 with scales).
 
 Every function runs on the tensors' GPU stream through libkda_mi355x.so and
 returns new tensors; there is no CPU fallback.  Arithmetic is f32 (f64 for
@@ -576,4 +578,134 @@ class _RMSNormGate(torch.autograd.Function):
                 dgl if gate_logits is not None and ctx.needs_input_grad[2] else None, None, None)
 
 
-__all__ = ["beta_gate", "chunkwise_kda_with_decay", "conv_silu", "lower_bounded_decay", "rmsnorm_gate"]
+def _check_add_norm(x, residual, weight, eps, dtypes) -> None:
+    if x.ndim < 1 or x.shape[-1] == 0:
+        raise ValueError(f"x must have shape [..., D] with D > 0, got {tuple(x.shape)}")
+    if x.dtype not in dtypes:
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError(f"residual must have shape {tuple(x.shape)}, got {tuple(residual.shape)}")
+        _check_dtype("residual", residual, x.dtype)
+        _check_device("residual", residual, x.device)
+    if weight is not None:
+        if weight.shape != (x.shape[-1],):
+            raise ValueError(f"weight must have shape [{x.shape[-1]}], got {tuple(weight.shape)}")
+        _check_dtype("weight", weight, x.dtype)
+        _check_device("weight", weight, x.device)
+    if not eps > 0:
+        raise ValueError("eps must be > 0")
+    _lib.require_gpu(x)
+
+
+def add_rmsnorm(
+    x: torch.Tensor,
+    residual: torch.Tensor | None = None,
+    weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(y, h)``: the sum ``h = x + residual`` of ``[..., D]`` tensors of one dtype
+    (``h`` is ``x`` itself without a residual) and its RMSNorm
+    ``y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension, ``weight [D]``
+    or None.  The norm reads the sum as it is stored, rounded to the dtype.
+    Differentiable in all tensors (``kda_add_rmsnorm_bwd``; the weight gradient
+    is summed in a fixed order)."""
+    _check_add_norm(x, residual, weight, eps, _DTYPES)
+    if _needs_grad(x, residual, weight):
+        y, h = _AddRMSNorm.apply(x, residual, weight, float(eps))
+    else:
+        y, h = _add_norm_forward(x, residual, weight, float(eps))
+    return y, (x if residual is None else h)
+
+
+def _add_norm_forward(x, residual, weight, eps):
+    xc = x.contiguous()
+    y = torch.empty_like(xc)
+    h = None if residual is None else torch.empty_like(xc)
+    if xc.numel():
+        rc = None if residual is None else residual.contiguous()
+        wc = None if weight is None else weight.contiguous()
+        with _prep.on_device(x.device):
+            _lib.check(_lib.load().kda_add_rmsnorm_fwd(
+                xc.data_ptr(), _lib.ptr(rc), _lib.ptr(wc), _lib.ptr(h), y.data_ptr(), xc.numel() // x.shape[-1],
+                x.shape[-1], eps, _lib.dtype_code(x.dtype), _prep.stream(x.device)))
+    return y, h
+
+
+class _AddRMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps):
+        y, h = _add_norm_forward(x, residual, weight, eps)
+        ctx.save_for_backward(x if h is None else h, weight)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh):
+        h, weight = ctx.saved_tensors
+        need_x, need_r, need_w, _ = ctx.needs_input_grad
+        if dy is None:  # the norm's output was not used
+            return dh if need_x else None, dh if need_r else None, None, None
+        width = h.shape[-1]
+        hc, dyc = h.contiguous(), dy.to(h.dtype).contiguous()
+        dx = torch.empty_like(hc)
+        dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_w else None
+        if hc.numel() == 0:
+            dw = None if dw is None else dw.zero_()
+        else:
+            dhc = None if dh is None else dh.to(h.dtype).contiguous()
+            wc = None if weight is None else weight.contiguous()
+            lib, rows, code = _lib.load(), hc.numel() // width, _lib.dtype_code(h.dtype)
+            with _prep.on_device(h.device):
+                nbytes = lib.kda_add_rmsnorm_bwd_workspace_bytes(rows, width, code) if need_w else 0
+                workspace = _prep.workspace(nbytes, h.device, "the add_rmsnorm backward")
+                _lib.check(lib.kda_add_rmsnorm_bwd(
+                    hc.data_ptr(), _lib.ptr(wc), dyc.data_ptr(), _lib.ptr(dhc), dx.data_ptr(), _lib.ptr(dw), rows,
+                    width, ctx.eps, code, _lib.ptr(workspace), nbytes, _prep.stream(h.device)))
+        return dx if need_x else None, dx if need_r else None, dw, None
+
+
+_GROUPS = (32, 64, 128, 256)
+
+
+def add_rmsnorm_quant(
+    x: torch.Tensor,
+    residual: torch.Tensor | None = None,
+    weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    *,
+    group_size: int | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(q, scales, h)``: ``add_rmsnorm`` with ``y`` in 8 bits, ``y ~ q * scales``:
+    ``q [..., D]`` in ``torch.float8_e4m3fn``, and f32 scales of one row
+    (``[..., 1]``) or of ``group_size`` (32, 64, 128 or 256, a divisor of D)
+    neighbouring elements (``[..., D / group_size]``), each the group's largest
+    magnitude over 448; the quotient is rounded once, from f32.  A group whose
+    largest magnitude is under 2^-100 reads back as zeros, one with a NaN as
+    NaN.  bf16, f16 and f32 tensors, for serving: it has no gradient and
+    raises for tensors that need one."""
+    _check_add_norm(x, residual, weight, eps, (torch.bfloat16, torch.float16, torch.float32))
+    width = x.shape[-1]
+    if group_size is not None and (group_size not in _GROUPS or width % group_size != 0):
+        raise ValueError(f"group_size must be one of {_GROUPS} and divide {width}, got {group_size}")
+    if _needs_grad(x, residual, weight):
+        raise RuntimeError("add_rmsnorm_quant has no backward; use add_rmsnorm, or call it under torch.no_grad()")
+    group = width if group_size is None else group_size
+    xc = x.contiguous()
+    q = torch.empty_like(xc, dtype=torch.float8_e4m3fn)
+    scales = torch.empty(*x.shape[:-1], width // group, dtype=torch.float32, device=x.device)
+    h = None if residual is None else torch.empty_like(xc)
+    if xc.numel():
+        rc = None if residual is None else residual.contiguous()
+        wc = None if weight is None else weight.contiguous()
+        with _prep.on_device(x.device):
+            _lib.check(_lib.load().kda_add_rmsnorm_quant(
+                xc.data_ptr(), _lib.ptr(rc), _lib.ptr(wc), _lib.ptr(h), q.data_ptr(), scales.data_ptr(), group,
+                xc.numel() // width, width, float(eps), _lib.dtype_code(x.dtype), _prep.stream(x.device)))
+    return q, scales, (x if residual is None else h)
+
+
+__all__ = ["add_rmsnorm", "add_rmsnorm_quant", "beta_gate", "chunkwise_kda_with_decay", "conv_silu",
+           "lower_bounded_decay", "rmsnorm_gate"]

@@ -554,3 +554,36 @@ def kda_layer(w, x, attention_mask=None, state=None, mode="chunkwise", output_fi
         offset = lengths if state is None else state[4] + lengths
         nxt = (final, qn, kn, vn, offset)
     return out, nxt
+
+
+# ---- the residual's addition and RMSNorm --------------------------------------
+
+
+def add_rmsnorm(x, residual=None, weight=None, eps=1e-6):
+    """``(y, h)``, y in f64 from the stored sum h (in x's dtype)."""
+    h = x if residual is None else (x.double() + residual.double()).to(x.dtype)
+    hd = h.double()
+    y = hd / torch.sqrt(hd.square().mean(-1, keepdim=True) + eps)
+    return (y if weight is None else y * weight.double()), h
+
+
+def add_rmsnorm_backward(h, weight, dy, dh, eps=1e-6):
+    """``(dx, dw)`` in f64: the gradients of the sum's two terms (alike) and of the weight."""
+    hd, dyd = h.double(), dy.double()
+    s = 1 / torch.sqrt(hd.square().mean(-1, keepdim=True) + eps)
+    wdy = dyd if weight is None else dyd * weight.double()
+    dx = s * (wdy - hd * s.square() * (wdy * hd).mean(-1, keepdim=True))
+    if dh is not None:
+        dx = dx + dh.double()
+    return dx, (dyd * hd * s).reshape(-1, h.shape[-1]).sum(0)
+
+
+def e4m3_groups(y, group):
+    """``(quotients, scales)`` in f64 of y's groups: what the e4m3 values are rounded from."""
+    blocks = y.unflatten(-1, (-1, group))
+    amax = blocks.abs().amax(-1)
+    zero = amax < 2.0 ** -100
+    scales = torch.where(zero, torch.zeros_like(amax), amax / 448)
+    quotients = torch.where(zero[..., None], torch.zeros_like(blocks),
+                            blocks / torch.where(zero, torch.ones_like(amax), scales)[..., None])
+    return quotients.flatten(-2), scales
