@@ -546,6 +546,52 @@ int kda_add_rmsnorm_bwd(const void* h, const void* weight, const void* d_y, cons
                         int64_t rows, int64_t width, double eps, int dtype, void* workspace, size_t workspace_bytes,
                         void* stream);
 
+/*
+ * Decode caches into and out of 8-bit pools, many tensors in one launch per 64.  Entry i < n
+ * goes from source entry src_index[i] (i when NULL) to destination entry dst_index[i] (i when
+ * NULL); both are device int64 [n], the sources hold n_src and the destinations n_dst entries.
+ *   KDA_MOVE_PACK   : src [n_src, rows, width] of `dtype` (f32, f16 or bf16) to dst int8
+ *                     [n_dst, rows, width] and scales [n_dst, rows]:
+ *                     scale = max|row| / 127, q = round_half_even(row / scale); a row whose
+ *                     largest magnitude is under 2^-100 is held as zeros with scale 0, one
+ *                     with a value that is not finite as zeros with scale NaN
+ *   KDA_MOVE_UNPACK : src int8 [n_src, rows, width] and scales [n_src, rows] to dst of `dtype`
+ *                     [n_dst, rows, width], q * scale
+ *   KDA_MOVE_BYTES  : `width` bytes per entry, any type (rows: 1)
+ * status (device int32 or NULL) is set to 1, never cleared, when an index is out of range; such
+ * a destination is not written, and from such a source come NaN (UNPACK), zeros (BYTES) or
+ * nothing (PACK).  A destination entry that is named twice takes the last one; the others stay
+ * as they were.  What is written may not overlap anything else.  `tensors` is read before the
+ * call returns.
+ */
+#define KDA_MOVE_BYTES 0
+#define KDA_MOVE_PACK 1
+#define KDA_MOVE_UNPACK 2
+
+typedef struct {
+  const void* src;
+  void* dst;
+  float* scales;
+  int64_t rows, width;
+  int kind;
+} kda_state_tensor;
+
+int kda_state_move(const kda_state_tensor* tensors, int count, int dtype, const int64_t* src_index, int64_t n_src,
+                   const int64_t* dst_index, int64_t n_dst, int64_t n, int* status, void* stream);
+
+/*
+ * kda_recurrent_fwd from 8-bit initial states (f32, f16 or bf16 inputs, f32 arithmetic):
+ *   values, scales : int8 [num_slots, heads, key_dim, value_dim], f32 [num_slots, heads, key_dim]
+ *   slots          : device int64 [num_seqs], the entry each sequence starts from, or NULL (its
+ *                    own number); a sequence whose entry does not exist starts from NaN
+ *   final_state    : f32 [num_seqs, heads, key_dim, value_dim] or NULL
+ */
+int kda_recurrent_fwd_packed(const void* q, const void* k, const void* v, const void* g, const void* beta,
+                             int in_dtype, const int8_t* values, const float* scales, const int64_t* slots,
+                             int64_t num_slots, float* final_state, void* out, const int32_t* cu_seqlens,
+                             int64_t dense_span, const int32_t* valid_lens, int64_t num_seqs, int64_t total_tokens,
+                             int64_t heads, int64_t key_dim, int64_t value_dim, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -716,4 +716,43 @@ int kda_add_rmsnorm_bwd(const void* h, const void* weight, const void* d_y, cons
                              static_cast<hipStream_t>(stream));
 }
 
+int kda_state_move(const kda_state_tensor* tensors, int count, int dtype, const int64_t* src_index, int64_t n_src,
+                   const int64_t* dst_index, int64_t n_dst, int64_t n, int* status, void* stream) {
+  g_detail[0] = '\0';
+  if (dtype != KDA_DTYPE_F32 && dtype != KDA_DTYPE_F16 && dtype != KDA_DTYPE_BF16) {
+    set_detail("state_move: states of f32, f16 or bf16 (dtype %d)", dtype);
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  if (count < 0 || (count > 0 && !tensors) || n < 0 || n > 0x7fffffffLL || n_src < 0 || n_dst < 0) {
+    set_detail("state_move: bad tensor or entry count");
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  if ((!src_index && n > n_src) || (!dst_index && n > n_dst) || (n > 0 && (n_src == 0 || n_dst == 0))) {
+    set_detail("state_move: %lld entries from %lld to %lld", (long long)n, (long long)n_src, (long long)n_dst);
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  if (n == 0) return KDA_OK;
+  return launch_state_move(tensors, count, dtype, src_index, n_src, dst_index, n_dst, n, status,
+                           static_cast<hipStream_t>(stream));
+}
+
+int kda_recurrent_fwd_packed(const void* q, const void* k, const void* v, const void* g, const void* beta,
+                             int in_dtype, const int8_t* values, const float* scales, const int64_t* slots,
+                             int64_t num_slots, float* final_state, void* out, const int32_t* cu_seqlens,
+                             int64_t dense_span, const int32_t* valid_lens, int64_t num_seqs, int64_t total_tokens,
+                             int64_t heads, int64_t key_dim, int64_t value_dim, void* stream) {
+  int rc = check_common(q, k, v, g, beta, in_dtype, KDA_DTYPE_F32, out, num_seqs, total_tokens, heads, key_dim,
+                        value_dim);
+  if (rc != KDA_OK) return rc;
+  rc = check_seq(cu_seqlens, dense_span, num_seqs, total_tokens);
+  if (rc != KDA_OK) return rc;
+  if (!values || !scales || num_slots <= 0 || (!slots && num_slots < num_seqs)) {
+    set_detail("recurrent_fwd_packed: values and scales must be non-null, with an entry for every sequence");
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  return launch_recurrent_packed(q, k, v, g, beta, in_dtype, values, scales, slots, num_slots, final_state, out,
+                                 kda::SeqDesc{cu_seqlens, dense_span, valid_lens}, num_seqs, heads, key_dim, value_dim,
+                                 static_cast<hipStream_t>(stream));
+}
+
 }  // extern "C"

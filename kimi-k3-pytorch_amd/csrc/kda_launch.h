@@ -173,4 +173,14 @@ size_t add_norm_bwd_workspace_bytes(int64_t rows, int64_t width, int dtype);
 int launch_add_norm_bwd(const void* h, const void* w, const void* dy, const void* dh, void* dx, void* dw, int64_t rows,
                         int64_t width, double eps, int dtype, void* workspace, hipStream_t stream);
 
+// Decode caches into and out of 8-bit pools (csrc/kda_state_pack.hip).
+int launch_state_move(const kda_state_tensor* tensors, int count, int dtype, const int64_t* src_index, int64_t n_src,
+                      const int64_t* dst_index, int64_t n_dst, int64_t n, int* status, hipStream_t stream);
+
+// The recurrence from 8-bit states (csrc/kda_recurrent.hip).
+int launch_recurrent_packed(const void* q, const void* k, const void* v, const void* g, const void* beta, int in_dtype,
+                            const int8_t* values, const float* scales, const int64_t* slots, int64_t n_slots,
+                            float* s_out, void* out, const kda::SeqDesc& seq, int64_t N, int64_t H, int64_t K,
+                            int64_t V, hipStream_t stream);
+
 }  // namespace kda_host

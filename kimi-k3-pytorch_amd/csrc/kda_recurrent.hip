@@ -31,6 +31,13 @@ struct RecArgs {
   ST* s_hist;  // [T, N, H, K, V] or nullptr
   SeqDesc seq;
   int64_t N, H, K, V;
+  // 8-bit initial states in place of s_in: values [n_slots, H, K, V] and row scales
+  // [n_slots, H, K]; sequence s starts from entry slots[s] (s without slots), from
+  // NaN where there is no such entry
+  const int8_t* p_in;
+  const float* p_scales;
+  const int64_t* slots;
+  int64_t n_slots;
 };
 
 template <int N, class T>
@@ -75,7 +82,8 @@ __device__ __forceinline__ void store_state_row(ST* p, const ST (&src)[VPT]) {
 }
 
 // FULL: K == TK*KPT and V % (TV*VPT) == 0, all accesses in range without checks.
-template <class IT, class ST, int TK, int KPT, int TV, int VPT, bool FULL, bool NT>
+// PACKED: the initial state is held in 8 bits.
+template <class IT, class ST, int TK, int KPT, int TV, int VPT, bool FULL, bool NT, bool PACKED = false>
 __global__ __launch_bounds__(TK* TV) void recurrent_kernel(const RecArgs<IT, ST> a) {
   constexpr int VT = TV * VPT;
   __shared__ ST red_r[2][TK][VT];
@@ -100,19 +108,40 @@ __global__ __launch_bounds__(TK* TV) void recurrent_kernel(const RecArgs<IT, ST>
   auto col_ok = [&](int j) -> bool { return FULL || (vcol0 + j) < a.V; };
 
   ST st[KPT][VPT];
+  if constexpr (PACKED) {
+    const int64_t slot = a.slots != nullptr ? a.slots[s] : s;
+    const bool there = slot >= 0 && slot < a.n_slots;
+    const int64_t row0 = ((there ? slot : 0) * a.H + h) * a.K + k0;
 #pragma unroll
-  for (int i = 0; i < KPT; ++i) {
-    if (a.s_in != nullptr && row_ok(i)) {
-      const ST* p = a.s_in + state_base + static_cast<int64_t>(k0 + i) * a.V + vcol0;
-      if (FULL) {
-        load_state_row<ST, VPT, NT>(p, st[i]);
+    for (int i = 0; i < KPT; ++i) {
+      ST scale = ST(0);
+      if (row_ok(i)) scale = there ? ST(a.p_scales[row0 + i]) : ST(__builtin_nanf(""));
+      if constexpr (FULL) {
+        typedef int8_t q_t __attribute__((ext_vector_type(VPT)));
+        const q_t q = __builtin_nontemporal_load(reinterpret_cast<const q_t*>(a.p_in + (row0 + i) * a.V + vcol0));
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) st[i][j] = static_cast<ST>(q[j]) * scale;
       } else {
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) st[i][j] = col_ok(j) ? p[j] : ST(0);
+        for (int j = 0; j < VPT; ++j)
+          st[i][j] = row_ok(i) && col_ok(j) ? static_cast<ST>(a.p_in[(row0 + i) * a.V + vcol0 + j]) * scale : ST(0);
       }
-    } else {
+    }
+  } else {
 #pragma unroll
-      for (int j = 0; j < VPT; ++j) st[i][j] = ST(0);
+    for (int i = 0; i < KPT; ++i) {
+      if (a.s_in != nullptr && row_ok(i)) {
+        const ST* p = a.s_in + state_base + static_cast<int64_t>(k0 + i) * a.V + vcol0;
+        if (FULL) {
+          load_state_row<ST, VPT, NT>(p, st[i]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < VPT; ++j) st[i][j] = col_ok(j) ? p[j] : ST(0);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) st[i][j] = ST(0);
+      }
     }
   }
 
@@ -229,7 +258,7 @@ __global__ __launch_bounds__(TK* TV) void recurrent_kernel(const RecArgs<IT, ST>
   }
 }
 
-template <class IT, class ST, int TK, int KPT, int TV, int VPT, bool FULL, bool NT>
+template <class IT, class ST, int TK, int KPT, int TV, int VPT, bool FULL, bool NT, bool PACKED = false>
 static int launch_cfg(const RecArgs<IT, ST>& a, hipStream_t stream) {
   constexpr int VT = TV * VPT;
   const int64_t nvt = (a.V + VT - 1) / VT;
@@ -239,7 +268,7 @@ static int launch_cfg(const RecArgs<IT, ST>& a, hipStream_t stream) {
     kda_host::set_detail("recurrent: grid of %lld workgroups is too large", (long long)blocks);
     return KDA_ERR_UNSUPPORTED;
   }
-  hipLaunchKernelGGL((recurrent_kernel<IT, ST, TK, KPT, TV, VPT, FULL, NT>), dim3(static_cast<unsigned>(blocks)),
+  hipLaunchKernelGGL((recurrent_kernel<IT, ST, TK, KPT, TV, VPT, FULL, NT, PACKED>), dim3(static_cast<unsigned>(blocks)),
                      dim3(TK * TV), 0, stream, a);
   return kda_host::check_launch("recurrent_kernel");
 }
@@ -263,7 +292,7 @@ template <class IT, class ST>
 static int run_typed(const void* q, const void* k, const void* v, const void* g, const void* beta,
                      const void* s_in, void* s_out, void* out, void* s_hist, const SeqDesc& seq,
                      int64_t N, int64_t H, int64_t K, int64_t V, hipStream_t stream, bool streaming_state) {
-  RecArgs<IT, ST> a;
+  RecArgs<IT, ST> a{};
   a.q = static_cast<const IT*>(q);
   a.k = static_cast<const IT*>(k);
   a.v = static_cast<const IT*>(v);
@@ -281,9 +310,49 @@ static int run_typed(const void* q, const void* k, const void* v, const void* g,
   return dispatch<IT, ST>(a, stream, streaming_state);
 }
 
+// The same from 8-bit states, f32 arithmetic.
+template <class IT>
+static int run_packed(const void* q, const void* k, const void* v, const void* g, const void* beta,
+                      const int8_t* values, const float* scales, const int64_t* slots, int64_t n_slots, float* s_out,
+                      void* out, const SeqDesc& seq, int64_t N, int64_t H, int64_t K, int64_t V, hipStream_t stream) {
+  RecArgs<IT, float> a{};
+  a.q = static_cast<const IT*>(q);
+  a.k = static_cast<const IT*>(k);
+  a.v = static_cast<const IT*>(v);
+  a.g = static_cast<const IT*>(g);
+  a.beta = static_cast<const IT*>(beta);
+  a.out = static_cast<IT*>(out);
+  a.s_out = s_out;
+  a.seq = seq;
+  a.N = N, a.H = H, a.K = K, a.V = V;
+  a.p_in = values, a.p_scales = scales, a.slots = slots, a.n_slots = n_slots;
+  const bool aligned = reinterpret_cast<uintptr_t>(values) % 4 == 0 && reinterpret_cast<uintptr_t>(s_out) % 16 == 0;
+  if (K == 128 && V % 128 == 0 && aligned) return launch_cfg<IT, float, 8, 16, 32, 4, true, true, true>(a, stream);
+  if (K <= 32) return launch_cfg<IT, float, 16, 2, 16, 1, false, false, true>(a, stream);
+  if (K <= 128) return launch_cfg<IT, float, 16, 8, 16, 1, false, false, true>(a, stream);
+  if (K <= 256) return launch_cfg<IT, float, 16, 16, 16, 1, false, false, true>(a, stream);
+  kda_host::set_detail("recurrent: key_dim %lld > 256 is not supported", (long long)K);
+  return KDA_ERR_UNSUPPORTED;
+}
+
 }  // namespace kda
 
 namespace kda_host {
+
+int launch_recurrent_packed(const void* q, const void* k, const void* v, const void* g, const void* beta, int in_dtype,
+                            const int8_t* values, const float* scales, const int64_t* slots, int64_t n_slots,
+                            float* s_out, void* out, const kda::SeqDesc& seq, int64_t N, int64_t H, int64_t K,
+                            int64_t V, hipStream_t stream) {
+  using namespace kda;
+  switch (in_dtype) {
+    case KDA_DTYPE_BF16:
+      return run_packed<bf16>(q, k, v, g, beta, values, scales, slots, n_slots, s_out, out, seq, N, H, K, V, stream);
+    case KDA_DTYPE_F16:
+      return run_packed<f16>(q, k, v, g, beta, values, scales, slots, n_slots, s_out, out, seq, N, H, K, V, stream);
+    default:
+      return run_packed<float>(q, k, v, g, beta, values, scales, slots, n_slots, s_out, out, seq, N, H, K, V, stream);
+  }
+}
 
 int launch_recurrent(const void* q, const void* k, const void* v, const void* g, const void* beta, int in_dtype,
                      const void* s_in, void* s_out, int state_dtype, void* out, void* s_hist,

@@ -10,15 +10,17 @@ All arithmetic runs in hand-written HIP kernels in ``libkda_mi355x.so``; see
 include/kda_mi355x.h for the C ABI.
 """
 
-from . import cache, fused, layer
+from . import cache, fused, layer, state
 from .chunkwise import chunkwise_kda
 from .recurrent import KDAOperatorOutput, recurrent_kda
-from .state import KDAState, ShortConvState
+from .state import KDAState, PackedKDAState, PackedState, ShortConvState
 from .ut_transform import UTTransformOutput, ut_transform
 
 __all__ = [
     "KDAOperatorOutput",
     "KDAState",
+    "PackedKDAState",
+    "PackedState",
     "ShortConvState",
     "UTTransformOutput",
     "cache",
@@ -26,5 +28,6 @@ __all__ = [
     "fused",
     "layer",
     "recurrent_kda",
+    "state",
     "ut_transform",
 ]

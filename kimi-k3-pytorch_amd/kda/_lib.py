@@ -51,6 +51,17 @@ class LayerDecodeArgs(ctypes.Structure):
     )
 
 
+class StateTensor(ctypes.Structure):
+    """kda_state_tensor, field for field."""
+
+    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("rows", ctypes.c_int64), ("width", ctypes.c_int64), ("kind", ctypes.c_int)]
+
+
+# kda_state_tensor.kind
+MOVE_BYTES, MOVE_PACK, MOVE_UNPACK = 0, 1, 2
+
+
 # Every exported symbol with (restype, argtypes); include/kda_mi355x.h is the source of truth.
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -112,6 +123,8 @@ SIGNATURES = {
     "kda_mask_lengths": (_I, [_P, _L, _L, _P, _P]),
     "kda_layer_decode_workspace_bytes": (_S, [_P]),
     "kda_layer_decode": (_I, [_P, _P]),
+    "kda_state_move": (_I, [_P, _I, _I, _P, _L, _P, _L, _L, _P, _P]),
+    "kda_recurrent_fwd_packed": (_I, [_P] * 5 + [_I, _P, _P, _P, _L, _P, _P, _P, _L, _P] + [_L] * 5 + [_P]),
     "kda_add_rmsnorm_fwd": (_I, [_P] * 5 + [_L, _L, ctypes.c_double, _I, _P]),
     "kda_add_rmsnorm_quant": (_I, [_P] * 6 + [_L, _L, _L, ctypes.c_double, _I, _P]),
     "kda_add_rmsnorm_bwd_workspace_bytes": (_S, [_L, _L, _I]),

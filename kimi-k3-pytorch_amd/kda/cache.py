@@ -13,6 +13,12 @@ launch per 64 tensors, each selected row read once and written once.
 ``reorder_states(states, indices)`` and ``clone_states(states)`` take a
 sequence of ``KDAState``; ``gather_rows`` is the tensor-level form.  GPU
 tensors only: without the HIP library these raise ``RuntimeError``.
+
+Sequences at rest (idle sessions, preempted requests, shared prompts) keep
+their states in 8 bits: ``pack_states`` writes the caches of every layer into
+slots of a pool (``packed_pool``), ``unpack_states`` reads slots back
+(``kda_state_move``, csrc/kda_state_pack.hip, one launch per 64 tensors), and
+``recurrent_kda`` and ``chunkwise_kda`` start straight from a ``PackedState``.
 """
 
 from __future__ import annotations
@@ -23,7 +29,7 @@ from collections.abc import Sequence
 import torch
 
 from . import _lib, _prep
-from .state import KDAState, ShortConvState
+from .state import KDAState, PackedKDAState, PackedState, ShortConvState
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -175,3 +181,251 @@ def clone_states(states: Sequence[KDAState]) -> list[KDAState]:
     flat = [t for s in states for t in _flatten(s)]
     out = gather_rows(flat, None)
     return [_rebuild(out[5 * i : 5 * i + 5]) for i in range(len(states))]
+
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _move(tensors: list[_lib.StateTensor], dtype: torch.dtype, device: torch.device, src_index, n_src, dst_index, n_dst,
+          n, report=True) -> torch.Tensor | None:
+    """``kda_state_move`` and the status it sets for a slot out of range (None
+    without slots, or into a graph, where no one can read it)."""
+    checked = (report and (src_index is not None or dst_index is not None)
+               and not torch.cuda.is_current_stream_capturing())
+    status = torch.zeros(1, dtype=torch.int32, device=device) if checked else None
+    if n and tensors:
+        _lib.check(_lib.load().kda_state_move((_lib.StateTensor * len(tensors))(*tensors), len(tensors),
+                                              _lib.dtype_code(dtype), _lib.ptr(src_index), n_src, _lib.ptr(dst_index),
+                                              n_dst, n, _lib.ptr(status), _prep.stream(device)))
+    return status
+
+
+def _check_slots(status: torch.Tensor | None, slots: int) -> None:
+    if status is not None and int(status.item()) != 0:
+        raise IndexError(f"slot out of range for a pool of {slots}")
+
+
+def _slots_arg(slots: torch.Tensor | None, device: torch.device) -> torch.Tensor | None:
+    if slots is None:
+        return None
+    if slots.ndim != 1 or slots.dtype != torch.long:
+        raise ValueError("slots must be a rank-1 torch.long tensor")
+    if slots.device != device:
+        raise ValueError("slots and state must be on the same device")
+    return slots.contiguous()
+
+
+def _bytes(src: torch.Tensor, dst: torch.Tensor) -> _lib.StateTensor:
+    entries = src.shape[0]
+    width = src.numel() // entries * src.element_size() if entries else 0
+    return _lib.StateTensor(src.data_ptr(), dst.data_ptr(), None, 1, width, _lib.MOVE_BYTES)
+
+
+def _one_device(tensors: Sequence[torch.Tensor]) -> torch.device:
+    device = tensors[0].device
+    for t in tensors:
+        _lib.require_gpu(t)
+        if t.device != device:
+            raise ValueError("all cache tensors must be on one device")
+    return device
+
+
+def pack_recurrent(state: torch.Tensor) -> PackedState:
+    """Recurrent states ``[B,H,K,V]`` (f32, f16 or bf16) in 8 bits.  Every row
+    ``(b,h,k)`` of V values has its own scale, its largest magnitude over 127,
+    and holds the nearest whole multiples of it (halves to even).  A row whose
+    largest magnitude is under 2^-100 reads back as zeros, one with a value
+    that is not finite as NaN.  No gradient: raises for a state that needs one."""
+    _check_packable([state])
+    _one_device([state])
+    out = _empty_packed(state, state.shape[0])
+    with _prep.on_device(state.device):
+        st = state.contiguous()
+        _move([_pack(st, out)], st.dtype, st.device, None, st.shape[0], None, st.shape[0], st.shape[0])
+    return out
+
+
+def unpack_recurrent(packed: PackedState, slots: torch.Tensor | None = None,
+                     dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """``values * scales`` of all entries, or of ``slots`` (a slot may be named
+    more than once), as ``[B,H,K,V]`` of ``dtype``.  A slot out of range raises
+    ``IndexError``; in a captured graph, which no one can ask, it reads as NaN."""
+    device = _one_device([packed.values])
+    _check_float(dtype)
+    slots = _slots_arg(slots, device)
+    entries, rest = packed.values.shape[0], packed.values.shape[1:]
+    n = entries if slots is None else slots.shape[0]
+    _check_entries(n, entries)
+    out = torch.empty(n, *rest, dtype=dtype, device=device)
+    with _prep.on_device(device):
+        _check_slots(_move([_unpack(packed, out)], dtype, device, slots, entries, None, n, n), entries)
+    return out
+
+
+def read_slots(packed: PackedState, slots: torch.Tensor | None) -> torch.Tensor:
+    """``unpack_recurrent`` to f32 for checked slots, without waiting for the GPU:
+    NaN for a slot out of range."""
+    entries = packed.values.shape[0]
+    n = entries if slots is None else slots.shape[0]
+    out = torch.empty(n, *packed.values.shape[1:], dtype=torch.float32, device=_one_device([packed.values]))
+    with _prep.on_device(out.device):
+        _move([_unpack(packed, out)], torch.float32, out.device, slots, entries, None, n, n, report=False)
+    return out
+
+
+def packed_pool(states: Sequence[KDAState], slots: int) -> list[PackedKDAState]:
+    """An empty pool of ``slots`` slots per layer (zero states), for the caches of
+    these layers and any batch size."""
+    pool = []
+    for s in states:
+        conv = lambda c: ShortConvState(c.buffer.new_zeros(slots, *c.buffer.shape[1:]))  # noqa: E731
+        shape = (slots, *s.recurrent_state.shape[1:])
+        packed = PackedState(s.recurrent_state.new_zeros(shape, dtype=torch.int8),
+                             s.recurrent_state.new_zeros(shape[:3], dtype=torch.float32))
+        pool.append(PackedKDAState(packed, conv(s.q_conv_state), conv(s.k_conv_state), conv(s.v_conv_state),
+                                   s.sequence_offset.new_zeros(slots)))
+    return pool
+
+
+def pack_states(states: Sequence[KDAState], *, out: Sequence[PackedKDAState] | None = None,
+                slots: torch.Tensor | None = None) -> list[PackedKDAState]:
+    """Every layer's decode caches with their recurrent states in 8 bits
+    (``pack_recurrent``), all tensors in one native pass.
+
+    Without ``out`` the result is new tensors of the caches' batch.  With a pool
+    in ``out`` (one ``PackedKDAState`` a layer) batch row i goes to slot
+    ``slots[i]`` (a rank-1 ``torch.long`` tensor; None: slot i, for a pool of the
+    batch's size) and the other slots stay as they are; a slot named twice takes
+    the last row.  A slot out of range raises ``IndexError`` (its row is written
+    nowhere; in a captured graph, which no one can ask, only that).  No
+    gradient: raises for states that need one."""
+    states = list(states)
+    if out is None and slots is not None:
+        raise ValueError("slots need a pool in `out`")
+    if out is not None and len(out) != len(states):
+        raise ValueError(f"the pool has {len(out)} layers, the caches {len(states)}")
+    if not states:
+        return []
+    flat = [t for s in states for t in _flatten(s)]
+    _check_packable([s.recurrent_state for s in states])
+    if torch.is_grad_enabled() and any(t.requires_grad for t in flat):
+        raise RuntimeError("pack_states has no backward; call it on detached states or under torch.no_grad()")
+    device = _one_device(flat)
+    batch, dtype = flat[0].shape[0], flat[0].dtype
+    if any(t.shape[0] != batch for t in flat):
+        raise ValueError("all cache tensors must share the batch size")
+    if any(s.recurrent_state.dtype != dtype for s in states):
+        raise TypeError("the recurrent states of all layers must share one dtype")
+    slots = _slots_arg(slots, device)
+    if slots is not None and slots.shape[0] != batch:
+        raise ValueError(f"slots must name a slot for each of {batch} batch rows, got {slots.shape[0]}")
+    if out is None:
+        out = []
+        for s in states:
+            conv = lambda c: ShortConvState(torch.empty_like(c.buffer, memory_format=torch.contiguous_format))  # noqa: E731
+            out.append(PackedKDAState(_empty_packed(s.recurrent_state, batch), conv(s.q_conv_state),
+                                      conv(s.k_conv_state), conv(s.v_conv_state),
+                                      torch.empty_like(s.sequence_offset, memory_format=torch.contiguous_format)))
+    out = list(out)
+    entries = out[0].recurrent.values.shape[0]
+    if slots is None and entries != batch:
+        raise ValueError(f"a batch of {batch} needs slots for a pool of {entries}")
+    _check_entries(batch, entries)
+    moves, keep = [], []
+    for s, p in zip(states, out):
+        src = [_rows(t) for t in _flatten(s)]
+        dst = _packed_parts(p)
+        keep.append(src)
+        if p.recurrent.values.shape != (entries, *src[0].shape[1:]):
+            raise ValueError(f"pool values must have shape {(entries, *src[0].shape[1:])}, "
+                             f"got {tuple(p.recurrent.values.shape)}")
+        for a, b in zip(src[1:], dst[1:]):
+            if b.shape != (entries, *a.shape[1:]) or b.dtype != a.dtype:
+                raise ValueError(f"pool tensors must have shape {(entries, *a.shape[1:])} and dtype {a.dtype}, "
+                                 f"got {tuple(b.shape)} and {b.dtype}")
+            if not b.is_contiguous():
+                raise ValueError("pool tensors must be contiguous")
+        if any(b.device != device for b in dst):
+            raise ValueError("pool and states must be on the same device")
+        moves.append(_pack(src[0], p.recurrent))
+        moves += [_bytes(a, b) for a, b in zip(src[1:], dst[1:])]
+    with _prep.on_device(device):
+        _check_slots(_move(moves, dtype, device, None, batch, slots, entries, batch), entries)
+    return out
+
+
+def unpack_states(packed: Sequence[PackedKDAState], slots: torch.Tensor | None = None,
+                  dtype: torch.dtype = torch.float32) -> list[KDAState]:
+    """The decode caches held in ``slots`` (all slots in order when None) of every
+    layer, the recurrent states as ``dtype``, in one native pass; the other
+    tensors bit for bit.  A slot may be named more than once; one out of range
+    raises ``IndexError`` (in a captured graph, which no one can ask, its states
+    are NaN)."""
+    packed = list(packed)
+    if not packed:
+        return []
+    _check_float(dtype)
+    parts = [_packed_parts(p) for p in packed]
+    device = _one_device([t for part in parts for t in part])
+    slots = _slots_arg(slots, device)
+    entries = parts[0][0].shape[0]
+    if any(part[0].shape[0] != entries for part in parts):
+        raise ValueError("all layers of a pool must share the number of slots")
+    n = entries if slots is None else slots.shape[0]
+    _check_entries(n, entries)
+    moves, outs, keep = [], [], []
+    for p, part in zip(packed, parts):
+        rest = [_rows(t) for t in part[1:]]
+        keep.append(rest)
+        new = [torch.empty(n, *p.recurrent.values.shape[1:], dtype=dtype, device=device)]
+        new += [t.new_empty(n, *t.shape[1:]) for t in rest]
+        moves.append(_unpack(p.recurrent, new[0]))
+        moves += [_bytes(a, b) for a, b in zip(rest, new[1:])]
+        outs.append(new)
+    with _prep.on_device(device):
+        status = _move(moves, dtype, device, slots, entries, None, n, n)
+        states = [_rebuild(new) for new in outs]  # while the GPU copies
+        _check_slots(status, entries)
+    return states
+
+
+def _check_float(dtype: torch.dtype) -> None:
+    if dtype not in _FLOATS:
+        raise TypeError(f"recurrent states are read as float32, float16 or bfloat16, not {dtype}")
+
+
+def _check_packable(states: list[torch.Tensor]) -> None:
+    for state in states:
+        if state.ndim != 4:
+            raise ValueError(f"recurrent states must have shape [B,H,K,V], got {tuple(state.shape)}")
+        if state.dtype not in _FLOATS:
+            raise TypeError(f"recurrent states of float32, float16 or bfloat16 are packed, not {state.dtype}")
+        if torch.is_grad_enabled() and state.requires_grad:
+            raise RuntimeError("packing has no backward; pack a detached state or call it under torch.no_grad()")
+
+
+def _check_entries(n: int, entries: int) -> None:
+    if n and not entries:
+        raise IndexError("slot out of range for an empty pool")
+
+
+def _empty_packed(state: torch.Tensor, entries: int) -> PackedState:
+    shape = (entries, *state.shape[1:])
+    return PackedState(torch.empty(shape, dtype=torch.int8, device=state.device),
+                       torch.empty(shape[:3], dtype=torch.float32, device=state.device))
+
+
+def _pack(src: torch.Tensor, dst: PackedState) -> _lib.StateTensor:
+    _, heads, key_dim, value_dim = dst.values.shape
+    return _lib.StateTensor(src.data_ptr(), dst.values.data_ptr(), dst.scales.data_ptr(), heads * key_dim, value_dim,
+                            _lib.MOVE_PACK)
+
+
+def _unpack(src: PackedState, dst: torch.Tensor) -> _lib.StateTensor:
+    _, heads, key_dim, value_dim = src.values.shape
+    return _lib.StateTensor(src.values.data_ptr(), dst.data_ptr(), src.scales.data_ptr(), heads * key_dim, value_dim,
+                            _lib.MOVE_UNPACK)
+
+
+def _packed_parts(p: PackedKDAState) -> list[torch.Tensor]:
+    return [p.recurrent.values, p.q_conv_state.buffer, p.k_conv_state.buffer, p.v_conv_state.buffer, p.sequence_offset]

@@ -9,9 +9,10 @@ tests/kda/test_kda_chunkwise_equivalence.py:42-57 and
 tests/kda/test_kda_ut_transform.py:94-103), so both are validated exactly as
 the reference does and otherwise only select nothing.
 
-Additive keyword-only extension: ``cu_seqlens`` (packed documents
+Additive keyword-only extensions: ``cu_seqlens`` (packed documents
 ``[1, sum T, H, *]``, state reset at every document start, per-document
-``initial_state``/``final_state`` of shape ``[N,H,K,V]``).
+``initial_state``/``final_state`` of shape ``[N,H,K,V]``); and a ``PackedState``
+as ``initial_state``.
 
 Gradients: with autograd enabled and an input that requires grad, the call
 goes through ``_ChunkwiseFunction``, whose backward is the HIP chunk backward
@@ -41,7 +42,8 @@ import numpy as np
 import torch
 
 from . import _lib, _prep
-from .recurrent import KDAOperatorOutput
+from .recurrent import KDAOperatorOutput, checked_slots, read_packed
+from .state import PackedState
 from .utils import accumulation_dtype, checked_lengths, validate_core_inputs, validate_cu_seqlens
 
 
@@ -51,7 +53,7 @@ def chunkwise_kda(
     v: torch.Tensor,
     g: torch.Tensor,
     beta: torch.Tensor,
-    initial_state: torch.Tensor | None = None,
+    initial_state: torch.Tensor | PackedState | None = None,
     output_final_state: bool = False,
     attention_mask: torch.Tensor | None = None,
     *,
@@ -59,8 +61,13 @@ def chunkwise_kda(
     secondary_tile_size: int = 16,
     accumulate_state_in_fp32: bool = True,
     cu_seqlens: torch.Tensor | list[int] | None = None,
+    state_slots: torch.Tensor | None = None,
 ) -> KDAOperatorOutput:
-    """Exact chunkwise KDA using UT/WY parallel computation within each chunk."""
+    """Exact chunkwise KDA using UT/WY parallel computation within each chunk.
+
+    With a ``PackedState`` (states held in 8 bits, ``kda.cache``) sequence i starts
+    from entry ``state_slots[i]`` (None: entry i), read into f32 first; a slot out
+    of range gives that sequence NaN."""
     if chunk_size <= 0 or secondary_tile_size <= 0:
         raise ValueError("chunk_size and secondary_tile_size must be > 0")
     if secondary_tile_size > chunk_size:
@@ -70,7 +77,14 @@ def chunkwise_kda(
         offsets = validate_cu_seqlens(cu_seqlens, q.shape[0] if q.ndim == 4 else -1,
                                       q.shape[1] if q.ndim == 4 else -1, attention_mask)
     num_states = None if offsets is None else len(offsets) - 1
-    batch, tokens, *_ = validate_core_inputs(q, k, v, g, beta, initial_state, None, num_states=num_states)
+    packed = initial_state if isinstance(initial_state, PackedState) else None
+    if packed is None and state_slots is not None:
+        raise ValueError("state_slots need a PackedState as initial_state")
+    batch, tokens, *_ = validate_core_inputs(q, k, v, g, beta, None if packed is not None else initial_state, None,
+                                             num_states=num_states)
+    if packed is not None:
+        initial_state = read_packed(packed, checked_slots(packed, state_slots, q, v,
+                                                          batch if num_states is None else num_states))
     valid = checked_lengths(attention_mask, batch, tokens, q.device)
     return checked_chunkwise(q, k, v, g, beta, initial_state, output_final_state, attention_mask, valid,
                              accumulate_state_in_fp32, offsets)

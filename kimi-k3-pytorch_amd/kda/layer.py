@@ -35,9 +35,10 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib, _prep, fused
+from .cache import unpack_states
 from .chunkwise import checked_chunkwise
 from .recurrent import checked_recurrent
-from .state import KDAState, ShortConvState
+from .state import KDAState, PackedKDAState, ShortConvState
 from .utils import checked_lengths, validate_core_inputs
 
 
@@ -282,7 +283,7 @@ def kda_attention_forward(
     w: KDALayerWeights,
     hidden_states: torch.Tensor,
     attention_mask: torch.Tensor | None = None,
-    state: KDAState | None = None,
+    state: KDAState | PackedKDAState | None = None,
     mode: Literal["recurrent", "chunkwise", "decode"] = "chunkwise",
     output_final_state: bool = False,
     *,
@@ -290,7 +291,9 @@ def kda_attention_forward(
 ) -> KDALayerOutput:
     """One KDA layer call, as ``KimiDeltaAttention.forward`` (src/kda/kda.py:98-183)
     without the diagnostics.  ``update_state_in_place`` (decode only) writes the
-    new recurrent state over ``state.recurrent_state`` instead of a new tensor."""
+    new recurrent state over ``state.recurrent_state`` instead of a new tensor.
+    A ``PackedKDAState`` (caches at rest, ``kda.cache.pack_states``) is read back
+    first; the next state is a ``KDAState``."""
     if hidden_states.ndim != 3 or hidden_states.shape[-1] != w.d_model:
         raise ValueError(f"hidden_states must have shape [B,T,{w.d_model}], got {tuple(hidden_states.shape)}")
     batch, tokens, _ = hidden_states.shape
@@ -300,6 +303,10 @@ def kda_attention_forward(
         raise ValueError(f"unsupported KDA mode {mode!r}")
     if mode == "decode" and tokens != 1:
         raise ValueError("decode mode requires exactly one token")
+    if isinstance(state, PackedKDAState):
+        if update_state_in_place:
+            raise ValueError("update_state_in_place needs a KDAState, not a PackedKDAState")
+        state = unpack_states([state])[0]
     valid = checked_lengths(attention_mask, batch, tokens, hidden_states.device)
     _validate_state(w, hidden_states, state)
     x = hidden_states

@@ -11,6 +11,9 @@ Additive keyword-only extensions (every existing call is unchanged):
   (which must already be contiguous and in the work dtype) and return it as
   ``final_state``; the default keeps the reference's functional update
   (src/kda/recurrent.py:50-59).
+* a ``PackedState`` as ``initial_state`` (states held in 8 bits, ``kda.cache``), with
+  ``state_slots`` naming the entry each sequence starts from: the kernel reads
+  the 8-bit rows themselves (``kda_recurrent_fwd_packed``).
 """
 
 from __future__ import annotations
@@ -20,6 +23,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib, _prep
+from .state import PackedState
 from .utils import accumulation_dtype, checked_lengths, validate_core_inputs, validate_cu_seqlens
 
 
@@ -39,7 +43,7 @@ def recurrent_kda(
     v: torch.Tensor,
     g: torch.Tensor,
     beta: torch.Tensor,
-    initial_state: torch.Tensor | None = None,
+    initial_state: torch.Tensor | PackedState | None = None,
     output_final_state: bool = False,
     attention_mask: torch.Tensor | None = None,
     *,
@@ -47,14 +51,34 @@ def recurrent_kda(
     return_states_per_token: bool = False,
     cu_seqlens: torch.Tensor | list[int] | None = None,
     update_state_in_place: bool = False,
+    state_slots: torch.Tensor | None = None,
 ) -> KDAOperatorOutput:
-    """Exact KDA recurrence with decay, delta update, then read-after-write."""
+    """Exact KDA recurrence with decay, delta update, then read-after-write.
+
+    With a ``PackedState``, sequence i starts from entry ``state_slots[i]`` (a
+    rank-1 ``torch.long`` tensor; None: entry i, for as many entries as
+    sequences) and ``final_state`` is a new tensor in the work dtype; the call
+    does not wait for the GPU, so a slot out of range gives that sequence NaN."""
     offsets = None
     if cu_seqlens is not None:
         offsets = validate_cu_seqlens(cu_seqlens, q.shape[0] if q.ndim == 4 else -1,
                                       q.shape[1] if q.ndim == 4 else -1, attention_mask)
     num_states = None if offsets is None else len(offsets) - 1
-    batch, tokens, *_ = validate_core_inputs(q, k, v, g, beta, initial_state, None, num_states=num_states)
+    packed = initial_state if isinstance(initial_state, PackedState) else None
+    if packed is None and state_slots is not None:
+        raise ValueError("state_slots need a PackedState as initial_state")
+    batch, tokens, *_ = validate_core_inputs(q, k, v, g, beta, None if packed is not None else initial_state, None,
+                                             num_states=num_states)
+    if packed is not None:
+        if update_state_in_place:
+            raise ValueError("update_state_in_place needs a float initial_state, not a PackedState")
+        state_slots = checked_slots(packed, state_slots, q, v, batch if num_states is None else num_states)
+        direct = (accumulation_dtype(v.dtype, accumulate_state_in_fp32) == torch.float32
+                  and not return_states_per_token and not _chunkwise.needs_grad(q, k, v, g, beta))
+        if direct:
+            valid = checked_lengths(attention_mask, batch, tokens, q.device)
+            return _resume(q, k, v, g, beta, packed, state_slots, output_final_state, valid, offsets)
+        initial_state = read_packed(packed, state_slots)
     valid = checked_lengths(attention_mask, batch, tokens, q.device)
     return checked_recurrent(q, k, v, g, beta, initial_state, output_final_state, attention_mask, valid,
                              accumulate_state_in_fp32, return_states_per_token, offsets, update_state_in_place)
@@ -134,6 +158,57 @@ def checked_recurrent(q, k, v, g, beta, initial_state, output_final_state, atten
     if hist is not None:
         states = tuple(x if x.dtype == work_dtype else x.to(work_dtype) for x in hist.unbind(0))
     return KDAOperatorOutput(hidden_states=hidden, final_state=final, states_per_token=states)
+
+
+def checked_slots(packed: PackedState, slots, q, v, count: int):
+    """The checks of ``initial_state`` for a ``PackedState``: ``slots`` for ``count`` sequences."""
+    expected = (q.shape[2], q.shape[3], v.shape[-1])
+    entries = packed.values.shape[0]
+    if packed.values.shape[1:] != expected:
+        raise ValueError(f"packed initial_state must have shape [N, {', '.join(map(str, expected))}], "
+                         f"got {tuple(packed.values.shape)}")
+    if packed.values.device != q.device:
+        raise ValueError("initial_state and inputs must be on the same device")
+    if slots is None:
+        if entries != count:
+            raise ValueError(f"{count} sequences need state_slots for a packed initial_state of {entries} entries")
+        return None
+    if slots.shape != (count,) or slots.dtype != torch.long:
+        raise ValueError(f"state_slots must be a torch.long tensor of shape {(count,)}")
+    if slots.device != q.device:
+        raise ValueError("state_slots and inputs must be on the same device")
+    if entries == 0:
+        raise IndexError("slot out of range for an empty pool")
+    return slots.contiguous()
+
+
+def read_packed(packed: PackedState, slots: torch.Tensor | None) -> torch.Tensor:
+    """The f32 states of checked slots, for the calls that need them as a tensor;
+    NaN for a slot out of range."""
+    from .cache import read_slots
+
+    return read_slots(packed, slots)
+
+
+def _resume(q, k, v, g, beta, packed, slots, output_final_state, valid, offsets) -> KDAOperatorOutput:
+    """The recurrence from 8-bit states, on checked inputs; f32 arithmetic."""
+    _lib.require_gpu(q)
+    batch, tokens, heads, key_dim, value_dim = (*q.shape, v.shape[-1])
+    device = q.device
+    (qc, kc, vc, gc, bc), kernel_dtype, _ = _prep.kernel_inputs(q, k, v, g, beta, torch.float32)
+    n_seq = batch if offsets is None else len(offsets) - 1
+    s_out = None
+    if output_final_state:
+        s_out = torch.empty(n_seq, heads, key_dim, value_dim, dtype=torch.float32, device=device)
+    out = torch.empty(batch, tokens, heads, value_dim, dtype=kernel_dtype, device=device)
+    cu = None if offsets is None else _prep.cu_tensor(offsets, device)
+    with _prep.on_device(device):
+        _lib.check(_lib.load().kda_recurrent_fwd_packed(
+            qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), gc.data_ptr(), bc.data_ptr(), _lib.dtype_code(kernel_dtype),
+            packed.values.data_ptr(), packed.scales.data_ptr(), _lib.ptr(slots), packed.values.shape[0],
+            _lib.ptr(s_out), out.data_ptr(), _lib.ptr(cu), tokens, _lib.ptr(valid), n_seq, batch * tokens, heads,
+            key_dim, value_dim, _prep.stream(device)))
+    return KDAOperatorOutput(hidden_states=out if out.dtype == v.dtype else out.to(v.dtype), final_state=s_out)
 
 
 class _RecurrentStatesFunction(torch.autograd.Function):

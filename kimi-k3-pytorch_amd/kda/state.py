@@ -94,3 +94,43 @@ class KDAState:
             v_conv_state=ShortConvState(pick(self.v_conv_state.buffer)),
             sequence_offset=pick(self.sequence_offset),
         )
+
+
+@dataclass
+class PackedState:
+    """Recurrent states in 8 bits: ``values`` int8 ``[N,H,K,V]`` and one f32 scale a
+    row, ``scales [N,H,K]``; row ``(n,h,k)`` stands for ``values * scales``."""
+
+    values: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self) -> None:
+        if self.values.ndim != 4 or self.values.dtype != torch.int8:
+            raise ValueError("packed values must be int8 with shape [N,H,K,V]")
+        if self.scales.shape != self.values.shape[:3] or self.scales.dtype != torch.float32:
+            raise ValueError(f"packed scales must be float32 with shape {tuple(self.values.shape[:3])}")
+        if self.scales.device != self.values.device:
+            raise ValueError("packed values and scales must be on the same device")
+        if not (self.values.is_contiguous() and self.scales.is_contiguous()):
+            raise ValueError("packed values and scales must be contiguous")
+
+
+@dataclass
+class PackedKDAState:
+    """A layer's decode caches at rest, or the slots of a pool of them: the
+    fields of ``KDAState`` with the recurrent states in 8 bits."""
+
+    recurrent: PackedState
+    q_conv_state: ShortConvState
+    k_conv_state: ShortConvState
+    v_conv_state: ShortConvState
+    sequence_offset: torch.Tensor
+
+    def __post_init__(self) -> None:
+        slots = self.recurrent.values.shape[0]
+        if self.sequence_offset.shape != (slots,):
+            raise ValueError(f"sequence_offset must have shape {(slots,)}, got {tuple(self.sequence_offset.shape)}")
+        if self.sequence_offset.dtype != torch.long:
+            raise TypeError("sequence_offset must use torch.long")
+        if any(c.buffer.shape[0] != slots for c in (self.q_conv_state, self.k_conv_state, self.v_conv_state)):
+            raise ValueError("all ShortConv states must match the packed states' slots")

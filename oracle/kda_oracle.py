@@ -587,3 +587,21 @@ def e4m3_groups(y, group):
     quotients = torch.where(zero[..., None], torch.zeros_like(blocks),
                             blocks / torch.where(zero, torch.ones_like(amax), scales)[..., None])
     return quotients.flatten(-2), scales
+
+
+# ---- states in 8 bits -----------------------------------------------------------
+
+
+def pack_rows(state):
+    """``(values, scales)``: int8 multiples of a scale per row of the last dimension.
+    The quotients are rounded from f64, where a quotient of two f32 numbers is
+    never on the wrong side of a tie."""
+    x = state.float()
+    amax = x.abs().amax(-1)
+    finite = torch.isfinite(x).all(-1)
+    zero = finite & (amax < 2.0 ** -100)
+    scales = torch.where(zero, torch.zeros_like(amax), amax / 127)
+    use = finite & ~zero
+    safe = torch.where(use, scales, torch.ones_like(scales)).double()
+    values = torch.round(torch.where(use[..., None], x, torch.zeros_like(x)).double() / safe[..., None])
+    return values.to(torch.int8), torch.where(finite, scales, torch.full_like(scales, float("nan")))

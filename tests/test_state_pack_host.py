@@ -1,0 +1,119 @@
+"""Argument checks of the 8-bit state cache (no GPU: every error is raised before a launch)."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import kda
+from kda import _lib, cache
+
+
+def _packed(n=3, heads=2, key_dim=4, value_dim=8):
+    return kda.PackedState(torch.zeros(n, heads, key_dim, value_dim, dtype=torch.int8), torch.zeros(n, heads, key_dim))
+
+
+def _state(batch=3, dtype=torch.float32):
+    conv = lambda: kda.ShortConvState(torch.zeros(batch, 3, 8))  # noqa: E731
+    return kda.KDAState(torch.zeros(batch, 2, 4, 8, dtype=dtype), conv(), conv(), conv(),
+                        torch.zeros(batch, dtype=torch.long))
+
+
+def test_packed_types():
+    with pytest.raises(ValueError):
+        kda.PackedState(torch.zeros(2, 2, 4, 8), torch.zeros(2, 2, 4))
+    with pytest.raises(ValueError):
+        kda.PackedState(torch.zeros(2, 2, 4, 8, dtype=torch.int8), torch.zeros(2, 2, 8))
+    with pytest.raises(ValueError):
+        kda.PackedState(torch.zeros(2, 2, 8, 4, dtype=torch.int8).transpose(2, 3), torch.zeros(2, 2, 4))
+    p, s = _packed(), _state()
+    with pytest.raises(ValueError):
+        kda.PackedKDAState(p, s.q_conv_state, s.k_conv_state, s.v_conv_state, torch.zeros(4, dtype=torch.long))
+    with pytest.raises(TypeError):
+        kda.PackedKDAState(p, s.q_conv_state, s.k_conv_state, s.v_conv_state, torch.zeros(3))
+    with pytest.raises(ValueError):
+        kda.PackedKDAState(p, kda.ShortConvState(torch.zeros(2, 3, 8)), s.k_conv_state, s.v_conv_state,
+                           torch.zeros(3, dtype=torch.long))
+
+
+def test_pack_and_unpack_checks():
+    with pytest.raises(ValueError):
+        cache.pack_recurrent(torch.zeros(2, 4, 8))
+    with pytest.raises(TypeError):
+        cache.pack_recurrent(torch.zeros(1, 2, 4, 8, dtype=torch.float64))
+    with pytest.raises(RuntimeError, match="backward"):
+        cache.pack_recurrent(torch.zeros(1, 2, 4, 8, requires_grad=True))
+    with pytest.raises(RuntimeError, match="GPU"):
+        cache.pack_recurrent(torch.zeros(1, 2, 4, 8))
+    with pytest.raises(RuntimeError, match="GPU"):
+        cache.unpack_recurrent(_packed())
+    with pytest.raises(RuntimeError, match="GPU"):
+        cache.pack_states([_state()])
+    with pytest.raises(ValueError):
+        cache.pack_states([_state()], slots=torch.zeros(3, dtype=torch.long))
+    with pytest.raises(ValueError):
+        cache.pack_states([_state()], out=[])
+    with pytest.raises(TypeError):
+        cache.unpack_states(cache.packed_pool([_state()], 2), dtype=torch.float64)
+    assert cache.pack_states([]) == [] and cache.unpack_states([]) == []
+    pool = cache.packed_pool([_state()], 5)
+    assert pool[0].recurrent.values.shape == (5, 2, 4, 8) and pool[0].sequence_offset.shape == (5,)
+
+
+@pytest.mark.parametrize("call", [kda.recurrent_kda, kda.chunkwise_kda])
+def test_packed_initial_state_checks(call):
+    q = torch.zeros(3, 1, 2, 4)
+    args = (q, q, torch.zeros(3, 1, 2, 8), q, torch.zeros(3, 1, 2))
+    with pytest.raises(ValueError, match="PackedState"):
+        call(*args, None, state_slots=torch.zeros(3, dtype=torch.long))
+    with pytest.raises(ValueError, match="shape"):
+        call(*args, _packed(value_dim=4))
+    with pytest.raises(ValueError, match="state_slots"):
+        call(*args, _packed(n=4))
+    with pytest.raises(ValueError, match="state_slots"):
+        call(*args, _packed(), state_slots=torch.zeros(2, dtype=torch.long))
+    with pytest.raises(ValueError, match="state_slots"):
+        call(*args, _packed(), state_slots=torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(IndexError):
+        call(*args, _packed(n=0), state_slots=torch.zeros(3, dtype=torch.long))
+    with pytest.raises(RuntimeError, match="GPU"):
+        call(*args, _packed())
+
+
+def test_packed_state_is_not_updated_in_place():
+    q = torch.zeros(3, 1, 2, 4)
+    with pytest.raises(ValueError, match="update_state_in_place"):
+        kda.recurrent_kda(q, q, torch.zeros(3, 1, 2, 8), q, torch.zeros(3, 1, 2), _packed(),
+                          update_state_in_place=True)
+
+
+def test_move_entry_point_rejects_bad_arguments():
+    lib, bad = _lib.load(), _lib.KDA_ERR_INVALID_ARGUMENT
+    a, b, c = 1 << 20, 2 << 20, 3 << 20  # stand-in addresses, never dereferenced
+
+    def move(src=a, dst=b, scales=c, rows=4, width=8, kind=_lib.MOVE_PACK, dtype=0, n_src=3, n_dst=3, n=3, count=1,
+             index=None):
+        t = (_lib.StateTensor * 1)(_lib.StateTensor(src, dst, scales, rows, width, kind))
+        return lib.kda_state_move(ctypes.addressof(t) if count else None, count, dtype, index, n_src, None, n_dst, n,
+                                  None, None)
+
+    for kw in (dict(src=None), dict(dst=None), dict(scales=None), dict(kind=5), dict(rows=-1), dict(width=-1),
+               dict(width=1 << 32), dict(dtype=3), dict(n=4), dict(n_src=2), dict(n_dst=2), dict(n_src=0, index=a),
+               dict(n=-1), dict(count=-1), dict(src=a + 2), dict(scales=c + 1), dict(dst=a), dict(scales=a + 32),
+               dict(dst=a + 200), dict(kind=_lib.MOVE_UNPACK, dst=b + 2), dict(kind=_lib.MOVE_BYTES, dst=a + 8),
+               dict(rows=1 << 40, width=1 << 30)):
+        assert move(**kw) == bad, kw
+    assert move(n=0) == _lib.KDA_OK and move(count=0) == _lib.KDA_OK
+    # two tensors that write one place
+    t = (_lib.StateTensor * 2)(_lib.StateTensor(a, b, None, 1, 8, 0), _lib.StateTensor(c, b + 8, None, 1, 8, 0))
+    assert lib.kda_state_move(ctypes.addressof(t), 2, 0, None, 3, None, 3, 3, None, None) == bad
+
+    def step(values=a, scales=a, slots=None, n_slots=3, dtype=2, q=a):
+        return lib.kda_recurrent_fwd_packed(q, a, a, a, a, dtype, values, scales, slots, n_slots, a, a, None, 1, None,
+                                            3, 3, 2, 128, 128, None)
+
+    for kw in (dict(values=None), dict(scales=None), dict(n_slots=2), dict(n_slots=0, slots=a), dict(dtype=3),
+               dict(q=None)):
+        assert step(**kw) == bad, kw
