@@ -592,6 +592,32 @@ int kda_recurrent_fwd_packed(const void* q, const void* k, const void* v, const 
                              int64_t dense_span, const int32_t* valid_lens, int64_t num_seqs, int64_t total_tokens,
                              int64_t heads, int64_t key_dim, int64_t value_dim, void* stream);
 
+/*
+ * Low-rank adapters of many requests beside a shared projection, f32, f16 or bf16 tensors:
+ *   y_m = bias + scaling_a b_a (a_a x_m),  a = ids[m / span]
+ * in f32, rounded once: the projection's product x W^T is added by the caller (a GEMM with
+ * beta = 1).  A row with a negative id gets the bias alone, one with an id >= adapters NaN.
+ *   x       : [rows, d_in];  y : [rows, d_out];  bias : [d_out] or NULL (zeros)
+ *   a       : [adapters, rank, d_in];  b : [adapters, d_out, rank]
+ *   scaling : f32 [adapters] or NULL (1)
+ *   ids     : int32 or int64 (ids_are_int64) [ceil(rows / span)], span >= 1 rows an id
+ *   rank 1..256;  workspace of kda_adapter_delta_workspace_bytes(args), 16-byte aligned
+ */
+typedef struct {
+  const void *x, *a, *b, *bias;
+  const float* scaling;
+  const void* ids;
+  void* y;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t rows, span, d_in, d_out, rank, adapters;
+  int dtype, ids_are_int64;
+} kda_adapter_args;
+
+size_t kda_adapter_delta_workspace_bytes(const kda_adapter_args* args);
+
+int kda_adapter_delta(const kda_adapter_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

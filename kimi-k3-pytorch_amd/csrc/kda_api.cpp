@@ -755,4 +755,38 @@ int kda_recurrent_fwd_packed(const void* q, const void* k, const void* v, const 
                                  static_cast<hipStream_t>(stream));
 }
 
+static bool adapter_sizes(const kda_adapter_args* d) {
+  const int64_t most = 0x7fffffffLL;
+  return d && d->rows > 0 && d->rows <= most && d->span > 0 && d->d_in > 0 && d->d_in <= 0xffffff && d->d_out > 0 &&
+         d->d_out <= 0xffffff && d->rank > 0 && d->rank <= 256 && d->adapters > 0 && d->adapters <= 0xffffff &&
+         (d->dtype == KDA_DTYPE_F32 || d->dtype == KDA_DTYPE_F16 || d->dtype == KDA_DTYPE_BF16);
+}
+
+size_t kda_adapter_delta_workspace_bytes(const kda_adapter_args* args) {
+  return adapter_sizes(args) ? adapter_delta_workspace_bytes(*args) : 0;
+}
+
+int kda_adapter_delta(const kda_adapter_args* args, void* stream) {
+  g_detail[0] = '\0';
+  if (!adapter_sizes(args)) {
+    set_detail("adapter_delta: positive sizes (widths and adapters below 2^24), rank up to 256, f32, f16 or bf16");
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  const kda_adapter_args& d = *args;
+  if (!d.x || !d.a || !d.b || !d.ids || !d.y) {
+    set_detail("adapter_delta: x, a, b, ids and y must be non-null");
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  const size_t need = adapter_delta_workspace_bytes(d);
+  if (!d.workspace || d.workspace_bytes < need) {
+    set_detail("adapter_delta: workspace of %zu bytes needed", need);
+    return KDA_ERR_WORKSPACE;
+  }
+  if (reinterpret_cast<uintptr_t>(d.workspace) % 16 != 0) {
+    set_detail("adapter_delta: the workspace must be 16-byte aligned");
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  return launch_adapter_delta(d, static_cast<hipStream_t>(stream));
+}
+
 }  // extern "C"

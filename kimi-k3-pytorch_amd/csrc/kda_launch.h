@@ -183,4 +183,9 @@ int launch_recurrent_packed(const void* q, const void* k, const void* v, const v
                             float* s_out, void* out, const kda::SeqDesc& seq, int64_t N, int64_t H, int64_t K,
                             int64_t V, hipStream_t stream);
 
+// Adapters of many requests beside a shared projection (csrc/kda_adapter.hip).
+size_t adapter_delta_workspace_bytes(const kda_adapter_args& d);
+
+int launch_adapter_delta(const kda_adapter_args& d, hipStream_t stream);
+
 }  // namespace kda_host

@@ -1,0 +1,140 @@
+"""Low-rank adapters of many requests beside a layer's shared projections.
+
+A serving batch shares the weights of a projection, and each request may bring
+a low-rank adapter of its own: row m of the batch is
+
+    y_m = W x_m + bias + scaling_a B_a (A_a x_m),   a = its request's adapter,
+
+``[out, rank]`` times ``[rank, in]`` beside the ``[out, in]`` weight.  The
+adapters that a server keeps loaded are held stacked (``AdapterStack``), a batch
+names one per request (a negative id: none).  ``adapter_linear`` is the
+projection with them; ``layer.kda_attention_forward`` takes the stacks of its
+projections as ``KDALayerAdapters``.  For serving: there is no backward.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib, _prep
+
+_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+MAX_RANK = 256
+
+
+@dataclass
+class AdapterStack:
+    """N adapters of one projection: ``a [N, rank, in]``, ``b [N, out, rank]`` and
+    the f32 factors ``scaling [N]`` (None: 1).  Adapters of a smaller rank are
+    padded with zeros."""
+
+    a: torch.Tensor
+    b: torch.Tensor
+    scaling: torch.Tensor | None = None
+
+    def __post_init__(self) -> None:
+        if self.a.ndim != 3 or self.b.ndim != 3 or 0 in self.a.shape or 0 in self.b.shape:
+            raise ValueError("adapters must have shapes a [N,rank,in] and b [N,out,rank]")
+        if self.a.shape[0] != self.b.shape[0] or self.a.shape[1] != self.b.shape[2]:
+            raise ValueError(f"a {tuple(self.a.shape)} and b {tuple(self.b.shape)} disagree on N or rank")
+        if self.a.shape[1] > MAX_RANK:
+            raise ValueError(f"adapters of rank up to {MAX_RANK}, got {self.a.shape[1]}")
+        if self.a.dtype != self.b.dtype or self.a.dtype not in _DTYPES:
+            raise TypeError(f"adapters must share one dtype of float32, float16 or bfloat16, "
+                            f"got {self.a.dtype} and {self.b.dtype}")
+        if self.a.device != self.b.device:
+            raise ValueError("a and b must be on the same device")
+        if self.scaling is not None:
+            if self.scaling.shape != self.a.shape[:1] or self.scaling.dtype != torch.float32:
+                raise ValueError(f"scaling must be float32 of shape {tuple(self.a.shape[:1])}")
+            if self.scaling.device != self.a.device:
+                raise ValueError("scaling and the adapters must be on the same device")
+
+
+def _check(x, weight, bias, stack, adapter_ids) -> int:
+    """Argument checks; the rows of x per id."""
+    if x.ndim < 2 or x.shape[-1] == 0:
+        raise ValueError(f"x must have shape [B,...,in], got {tuple(x.shape)}")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    if weight.ndim != 2 or weight.shape[1] != x.shape[-1] or weight.shape[0] == 0:
+        raise ValueError(f"weight must have shape [out,{x.shape[-1]}], got {tuple(weight.shape)}")
+    out = weight.shape[0]
+    if bias is not None and bias.shape != (out,):
+        raise ValueError(f"bias must have shape [{out}], got {tuple(bias.shape)}")
+    n, rank, d_in = stack.a.shape
+    if d_in != x.shape[-1] or stack.b.shape[1] != out:
+        raise ValueError(f"adapters {tuple(stack.a.shape)}, {tuple(stack.b.shape)} do not fit a weight "
+                         f"{tuple(weight.shape)}")
+    for name, t in (("weight", weight), ("bias", bias), ("the adapters", stack.a)):
+        if t is not None and t.dtype != x.dtype:
+            raise TypeError(f"{name} must have dtype {x.dtype}, got {t.dtype}")
+    if adapter_ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError("adapter_ids must be int32 or int64")
+    lead = x.shape[:-1]
+    if adapter_ids.ndim < 1 or adapter_ids.shape != lead[: adapter_ids.ndim]:
+        raise ValueError(f"adapter_ids must have the leading shape of x, {tuple(lead)} or a part of it from the left, "
+                         f"got {tuple(adapter_ids.shape)}")
+    for name, t in (("weight", weight), ("bias", bias), ("the adapters", stack.a), ("adapter_ids", adapter_ids)):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name} must be on {x.device}, got {t.device}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in
+                                       (x, weight, bias, stack.a, stack.b, stack.scaling)):
+        raise RuntimeError("adapter_linear has no backward; call it under torch.no_grad() or on detached tensors")
+    _lib.require_gpu(x)
+    return lead[adapter_ids.ndim:].numel()
+
+
+def adapter_linear(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    bias: torch.Tensor | None,
+    stack: AdapterStack,
+    adapter_ids: torch.Tensor,
+) -> torch.Tensor:
+    """``x @ weight.T + bias`` plus each row's adapter.
+
+    ``x [B,...,in]``; ``adapter_ids`` (int32 or int64, on the GPU) names the adapter of
+    each request, ``[B]``, or of each token, ``[B,T]`` (packed documents):
+    ``stack.a[id]`` and ``stack.b[id]``; a negative id has none.  The call does not
+    wait for the GPU, so an id past the stack cannot raise: its rows are NaN.
+    f32 accumulation, the adapter's part rounded to the dtype before the
+    projection's product is added to it."""
+    span = _check(x, weight, bias, stack, adapter_ids)
+    d_in, (d_out, rows) = x.shape[-1], (weight.shape[0], x.shape[:-1].numel())
+    y = torch.empty(*x.shape[:-1], d_out, dtype=x.dtype, device=x.device)
+    if rows == 0:
+        return y
+    xc, a, b, ids = (t.contiguous() for t in (x, stack.a, stack.b, adapter_ids))
+    bias = None if bias is None else bias.contiguous()
+    scaling = None if stack.scaling is None else stack.scaling.contiguous()
+    lib = _lib.load()
+    args = _lib.AdapterArgs(xc.data_ptr(), a.data_ptr(), b.data_ptr(), _lib.ptr(bias), _lib.ptr(scaling),
+                            ids.data_ptr(), y.data_ptr(), None, 0, rows, span, d_in, d_out, a.shape[1], a.shape[0],
+                            _lib.dtype_code(x.dtype), 1 if ids.dtype == torch.int64 else 0)
+    ref = ctypes.addressof(args)
+    with _prep.on_device(x.device):
+        args.workspace_bytes = lib.kda_adapter_delta_workspace_bytes(ref)
+        workspace = _prep.workspace(args.workspace_bytes, x.device, "adapter_linear")
+        args.workspace = _lib.ptr(workspace)
+        _lib.check(lib.kda_adapter_delta(ref, _prep.stream(x.device)))
+        y.view(rows, d_out).addmm_(xc.view(rows, d_in), weight.t())
+    return y
+
+
+@dataclass
+class KDALayerAdapters:
+    """The adapters of a KDA layer's projections (None: the projection has none);
+    one id per request picks the same entry of every stack."""
+
+    q_proj: AdapterStack | None = None
+    k_proj: AdapterStack | None = None
+    v_proj: AdapterStack | None = None
+    gate_proj: AdapterStack | None = None
+    output_proj: AdapterStack | None = None
+
+
+__all__ = ["AdapterStack", "KDALayerAdapters", "adapter_linear"]

@@ -35,6 +35,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib, _prep, fused
+from .adapters import KDALayerAdapters, adapter_linear
 from .cache import unpack_states
 from .chunkwise import checked_chunkwise
 from .recurrent import checked_recurrent
@@ -288,12 +289,16 @@ def kda_attention_forward(
     output_final_state: bool = False,
     *,
     update_state_in_place: bool = False,
+    adapters: KDALayerAdapters | None = None,
+    adapter_ids: torch.Tensor | None = None,
 ) -> KDALayerOutput:
     """One KDA layer call, as ``KimiDeltaAttention.forward`` (src/kda/kda.py:98-183)
     without the diagnostics.  ``update_state_in_place`` (decode only) writes the
     new recurrent state over ``state.recurrent_state`` instead of a new tensor.
     A ``PackedKDAState`` (caches at rest, ``kda.cache.pack_states``) is read back
-    first; the next state is a ``KDAState``."""
+    first; the next state is a ``KDAState``.  ``adapters`` with ``adapter_ids [B]``
+    adds each request's low-rank adapter to the projections (serving: no
+    gradients; ``adapters.adapter_linear``)."""
     if hidden_states.ndim != 3 or hidden_states.shape[-1] != w.d_model:
         raise ValueError(f"hidden_states must have shape [B,T,{w.d_model}], got {tuple(hidden_states.shape)}")
     batch, tokens, _ = hidden_states.shape
@@ -310,7 +315,16 @@ def kda_attention_forward(
     valid = checked_lengths(attention_mask, batch, tokens, hidden_states.device)
     _validate_state(w, hidden_states, state)
     x = hidden_states
-    if mode == "decode" and attention_mask is None:
+    if (adapters is None) != (adapter_ids is None):
+        raise ValueError("adapters and adapter_ids come together")
+    if adapter_ids is not None and adapter_ids.shape != (batch,):
+        raise ValueError(f"adapter_ids must have shape {(batch,)}, got {tuple(adapter_ids.shape)}")
+
+    def project(t, weight, bias, name):
+        stack = None if adapters is None else getattr(adapters, name)
+        return F.linear(t, weight, bias) if stack is None else adapter_linear(t, weight, bias, stack, adapter_ids)
+
+    if mode == "decode" and attention_mask is None and adapters is None:
         step = _decode_step(w, x, state, update_state_in_place)
         if step is not None:
             return step
@@ -321,11 +335,11 @@ def kda_attention_forward(
     qs, ks, vs = (None, None, None) if state is None else (state.q_conv_state, state.k_conv_state,
                                                              state.v_conv_state)
     conv = fused.conv_silu_with_lengths
-    q, q_next = conv(F.linear(x, w.q_proj, w.q_proj_bias), w.q_conv, w.q_conv_bias, qs, valid, num_heads=H,
+    q, q_next = conv(project(x, w.q_proj, w.q_proj_bias, "q_proj"), w.q_conv, w.q_conv_bias, qs, valid, num_heads=H,
                      normalize=True, eps=w.eps, output_final_state=return_state)
-    k, k_next = conv(F.linear(x, w.k_proj, w.k_proj_bias), w.k_conv, w.k_conv_bias, ks, valid, num_heads=H,
+    k, k_next = conv(project(x, w.k_proj, w.k_proj_bias, "k_proj"), w.k_conv, w.k_conv_bias, ks, valid, num_heads=H,
                      normalize=True, eps=w.eps, output_final_state=return_state)
-    v, v_next = conv(F.linear(x, w.v_proj, w.v_proj_bias), w.v_conv, w.v_conv_bias, vs, valid, num_heads=H,
+    v, v_next = conv(project(x, w.v_proj, w.v_proj_bias, "v_proj"), w.v_conv, w.v_conv_bias, vs, valid, num_heads=H,
                      normalize=False, eps=1e-6, output_final_state=return_state)
     beta_logits = F.linear(x, w.beta_proj, w.beta_bias)
     decay_logits = F.linear(F.linear(x, w.alpha_down), w.alpha_up).reshape(batch, tokens, H, K)
@@ -348,8 +362,8 @@ def kda_attention_forward(
 
     # RMSNorm x output gate, output projection, mask (src/kda/kda.py:153-161)
     gated = fused.rmsnorm_gate(core.hidden_states, w.norm_weight, w.eps,
-                               gate_logits=F.linear(x, w.gate_proj, w.gate_bias))
-    out = F.linear(gated.reshape(batch, tokens, H * V), w.output_proj, w.output_bias)
+                               gate_logits=project(x, w.gate_proj, w.gate_bias, "gate_proj"))
+    out = project(gated.reshape(batch, tokens, H * V), w.output_proj, w.output_bias, "output_proj")
     if attention_mask is not None:
         out = out * attention_mask[..., None].to(out.dtype)
 

@@ -605,3 +605,28 @@ def pack_rows(state):
     safe = torch.where(use, scales, torch.ones_like(scales)).double()
     values = torch.round(torch.where(use[..., None], x, torch.zeros_like(x)).double() / safe[..., None])
     return values.to(torch.int8), torch.where(finite, scales, torch.full_like(scales, float("nan")))
+
+
+# ---- low-rank adapters ------------------------------------------------------------
+
+
+def adapter_linear(x, weight, bias, a, b, scaling, ids):
+    """``(y, delta, terms)`` in f64 for ``x [rows, in]`` and an id per row: the projection
+    with each row's adapter, the adapter's part with the bias, and the sums of
+    magnitudes ``(projection, low-rank product, up-projection)`` that bound an f32 result."""
+    xd, wd = x.double(), weight.double()
+    bd = torch.zeros(weight.shape[0], dtype=torch.float64) if bias is None else bias.double()
+    delta = bd.repeat(x.shape[0], 1)
+    low, up = torch.zeros_like(delta), bd.abs().repeat(x.shape[0], 1)
+    for i, n in enumerate(ids.tolist()):
+        if n < 0:
+            continue
+        if n >= a.shape[0]:
+            delta[i] = float("nan")
+            continue
+        c = 1.0 if scaling is None else float(scaling[n])
+        s = a[n].double() @ xd[i]
+        delta[i] += c * (b[n].double() @ s)
+        up[i] += abs(c) * (b[n].double().abs() @ s.abs())
+        low[i] += abs(c) * (b[n].double().abs() @ (a[n].double().abs() @ xd[i].abs()))
+    return xd @ wd.T + delta, delta, (xd.abs() @ wd.abs().T, low, up)

@@ -1,0 +1,91 @@
+"""Argument checks of adapters (no GPU: every error is raised before a launch)."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from kda import _lib
+from kda.adapters import AdapterStack, KDALayerAdapters, adapter_linear
+from kda.layer import KDALayerWeights, kda_attention_forward
+from tests._inputs import layer_weights
+
+
+def _stack(n=2, rank=4, d_in=8, d_out=6, dtype=torch.float32):
+    return AdapterStack(torch.zeros(n, rank, d_in, dtype=dtype), torch.zeros(n, d_out, rank, dtype=dtype))
+
+
+def test_stack_checks():
+    z = torch.zeros
+    for a, b in ((z(2, 4), z(2, 6, 4)), (z(2, 4, 8), z(3, 6, 4)), (z(2, 4, 8), z(2, 6, 5)), (z(0, 4, 8), z(0, 6, 4)),
+                 (z(1, 257, 8), z(1, 6, 257))):
+        with pytest.raises(ValueError):
+            AdapterStack(a, b)
+    with pytest.raises(TypeError):
+        AdapterStack(z(2, 4, 8), z(2, 6, 4).half())
+    with pytest.raises(TypeError):
+        AdapterStack(z(2, 4, 8).double(), z(2, 6, 4).double())
+    for scaling in (z(3), z(2).double()):
+        with pytest.raises(ValueError):
+            AdapterStack(z(2, 4, 8), z(2, 6, 4), scaling)
+
+
+def test_call_checks():
+    x, w, bias, ids = torch.zeros(3, 5, 8), torch.zeros(6, 8), torch.zeros(6), torch.zeros(3, dtype=torch.long)
+    call = lambda x=x, w=w, bias=bias, stack=_stack(), ids=ids: adapter_linear(x, w, bias, stack, ids)  # noqa: E731
+    for kw in (dict(x=torch.zeros(8)), dict(x=torch.zeros(3, 5, 0)), dict(w=torch.zeros(6, 7)), dict(bias=torch.zeros(5)),
+               dict(stack=_stack(d_in=9)), dict(stack=_stack(d_out=7)), dict(ids=ids[:2]), dict(ids=ids[:, None].repeat(1, 4)),
+               dict(ids=torch.tensor(0))):
+        with pytest.raises(ValueError):
+            call(**kw)
+    for kw in (dict(x=x.double()), dict(w=w.half()), dict(bias=bias.half()), dict(stack=_stack(dtype=torch.bfloat16)),
+               dict(ids=ids.float())):
+        with pytest.raises(TypeError):
+            call(**kw)
+    with pytest.raises(RuntimeError, match="backward"):
+        call(w=w.clone().requires_grad_())
+    with pytest.raises(RuntimeError, match="backward"):
+        stack = _stack()
+        stack.a.requires_grad_()
+        call(stack=stack)
+    with pytest.raises(RuntimeError, match="GPU"):
+        call()
+
+
+def test_layer_checks():
+    weights = layer_weights(128, 1, 128, 128, dtype=torch.float32)
+    w = KDALayerWeights(**weights)
+    x = torch.zeros(2, 3, 128)
+    with pytest.raises(ValueError, match="together"):
+        kda_attention_forward(w, x, adapters=KDALayerAdapters())
+    with pytest.raises(ValueError, match="together"):
+        kda_attention_forward(w, x, adapter_ids=torch.zeros(2, dtype=torch.long))
+    with pytest.raises(ValueError, match="adapter_ids"):
+        kda_attention_forward(w, x, adapters=KDALayerAdapters(), adapter_ids=torch.zeros(3, dtype=torch.long))
+
+
+def test_entry_point_rejects_bad_arguments():
+    lib, p = _lib.load(), 4096
+
+    def args(**kw):
+        fields = dict(x=p, a=p, b=p, bias=None, scaling=None, ids=p, y=p, workspace=p, workspace_bytes=1 << 30, rows=4,
+                      span=1, d_in=8, d_out=8, rank=4, adapters=2, dtype=2, ids_are_int64=1)
+        return _lib.AdapterArgs(**{**fields, **kw})
+
+    def call(**kw):
+        d = args(**kw)
+        return lib.kda_adapter_delta(ctypes.addressof(d), None)
+
+    for kw in (dict(x=None), dict(a=None), dict(b=None), dict(ids=None), dict(y=None), dict(rows=0), dict(span=0),
+               dict(rows=1 << 31), dict(d_in=0), dict(d_in=1 << 24), dict(d_out=0), dict(rank=0), dict(rank=257),
+               dict(adapters=0), dict(dtype=3), dict(workspace=p + 4)):
+        assert call(**kw) == _lib.KDA_ERR_INVALID_ARGUMENT, kw
+    assert lib.kda_adapter_delta(None, None) == _lib.KDA_ERR_INVALID_ARGUMENT
+    d = args()
+    need = lib.kda_adapter_delta_workspace_bytes(ctypes.addressof(d))
+    assert need > 0
+    assert call(workspace=None) == _lib.KDA_ERR_WORKSPACE and call(workspace_bytes=need - 1) == _lib.KDA_ERR_WORKSPACE
+    d = args(rank=300)
+    assert lib.kda_adapter_delta_workspace_bytes(ctypes.addressof(d)) == 0
