@@ -552,7 +552,8 @@ int kda_add_rmsnorm_bwd(const void* h, const void* weight, const void* d_y, cons
  * NULL); both are device int64 [n], the sources hold n_src and the destinations n_dst entries.
  *   KDA_MOVE_PACK   : src [n_src, rows, width] of `dtype` (f32, f16 or bf16) to dst int8
  *                     [n_dst, rows, width] and scales [n_dst, rows]:
- *                     scale = max|row| / 127, q = round_half_even(row / scale); a row whose
+ *                     scale = max|row| * (1 / 127 in f32), q = round_half_even(row / scale) (the
+ *                     exact quotient); a row whose
  *                     largest magnitude is under 2^-100 is held as zeros with scale 0, one
  *                     with a value that is not finite as zeros with scale NaN
  *   KDA_MOVE_UNPACK : src int8 [n_src, rows, width] and scales [n_src, rows] to dst of `dtype`

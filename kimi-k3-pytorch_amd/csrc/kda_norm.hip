@@ -9,6 +9,8 @@
 // its quotients would leave f32.
 // Backward, with the gradients dy and dh of the two outputs:
 //   dx = dr = dh + s (w dy - h s^2 mean(w dy h)),  dw = sum over rows of dy h s.
+#include <initializer_list>
+
 #include "kda_launch.h"
 
 namespace kda {
@@ -104,6 +106,190 @@ __global__ __launch_bounds__(256) void add_norm_row_kernel(const AddNorm<T> a) {
   }
 }
 
+// Rows in registers: TPR threads a row (a wave with four rows a workgroup, or the
+// workgroup), NV vectors of 16 bytes a thread, every load of the row in flight
+// before the sum, one pass over memory.  FULL: widths of whole vectors at aligned
+// addresses; otherwise vectors load at element alignment (the hardware takes any
+// address) and the row's last one element by element.
+template <class T>
+struct NormVec {
+  static constexpr int N = 16 / sizeof(T);
+  typedef T type __attribute__((ext_vector_type(N)));
+  typedef T loose __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+
+template <class T, bool FULL>
+__device__ __forceinline__ typename NormVec<T>::type norm_load(const T* row, int i, int width) {
+  using V = NormVec<T>;
+  typename V::type v{};
+  const int c = i * V::N;
+  if constexpr (FULL) {
+    if (c < width) v = __builtin_nontemporal_load(reinterpret_cast<const typename V::type*>(row + c));
+  } else {
+    if (c + V::N <= width) {
+      v = *reinterpret_cast<const typename V::loose*>(row + c);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V::N; ++e)
+        if (c + e < width) v[e] = row[c + e];
+    }
+  }
+  return v;
+}
+
+template <class T, bool FULL>
+__device__ __forceinline__ void norm_store(T* row, int i, int width, typename NormVec<T>::type v) {
+  using V = NormVec<T>;
+  const int c = i * V::N;
+  if constexpr (FULL) {
+    if (c < width) __builtin_nontemporal_store(v, reinterpret_cast<typename V::type*>(row + c));
+  } else {
+    if (c + V::N <= width) {
+      *reinterpret_cast<typename V::loose*>(row + c) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V::N; ++e)
+        if (c + e < width) row[c + e] = v[e];
+    }
+  }
+}
+
+// Sum over the threads of a row (TPR == 64: the wave's).
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* part) {
+  v = group_sum<64>(v);
+  if constexpr (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int u = 0; u < TPR / 64; ++u) v += part[u];
+  }
+  return v;
+}
+
+template <class T, bool Q, bool FULL, int TPR, int NV>
+__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void add_norm_kernel(const AddNorm<T> a) {
+  using V = NormVec<T>;
+  constexpr int N = V::N;
+  __shared__ float part[TPR / 64], top[TPR / 64];
+  const int lane = TPR == 64 ? threadIdx.x & 63 : threadIdx.x;
+  const int64_t row = TPR == 64 ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (TPR == 64 && row >= a.rows) return;  // whole waves; no barrier follows
+  const int width = static_cast<int>(a.width);
+  const int64_t at = row * width;
+  typename V::type xv[NV], rv[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) xv[j] = norm_load<T, FULL>(a.x + at, lane + j * TPR, width);
+  float ss = 0.f;
+  if (a.r != nullptr) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) rv[j] = norm_load<T, FULL>(a.r + at, lane + j * TPR, width);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        xv[j][e] = from_compute<T>(to_float(static_cast<T>(xv[j][e])) + to_float(static_cast<T>(rv[j][e])));
+      norm_store<T, FULL>(a.h + at, lane + j * TPR, width, xv[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float h = to_float(static_cast<T>(xv[j][e]));
+      ss += h * h;
+    }
+  const float s = frsqrt(row_sum<TPR>(ss, part) / static_cast<float>(width) + a.eps);
+  float y[NV][N];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int i = lane + j * TPR;
+    typename V::type wv{};
+    if (a.w != nullptr) {
+      if constexpr (FULL) {
+        if (i * N < width) wv = *reinterpret_cast<const typename V::type*>(a.w + i * N);
+      } else {
+        wv = norm_load<T, false>(a.w, i, width);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      y[j][e] = to_float(static_cast<T>(xv[j][e])) * s;
+      if (a.w != nullptr) y[j][e] *= to_float(static_cast<T>(wv[e]));
+    }
+  }
+  if constexpr (!Q) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      typename V::type o;
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[e] = from_compute<T>(y[j][e]);
+      norm_store<T, FULL>(a.y + at, lane + j * TPR, width, o);
+    }
+  } else {
+    // lanes of a group; a row's single group: all of them
+    const bool whole = a.group == width;
+    const int lanes = whole ? 64 : static_cast<int>(a.group) / N;
+    float m[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      m[j] = 0.f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) m[j] = nan_max(fabsf(y[j][e]), m[j]);
+    }
+    if (whole) {
+#pragma unroll
+      for (int j = 1; j < NV; ++j) m[0] = nan_max(m[j], m[0]);
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) m[0] = nan_max(__shfl_xor(m[0], off), m[0]);
+      if constexpr (TPR > 64) {
+        if ((lane & 63) == 0) top[lane >> 6] = m[0];
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < TPR / 64; ++u) m[0] = nan_max(top[u], m[0]);
+      }
+#pragma unroll
+      for (int j = 1; j < NV; ++j) m[j] = m[0];
+    } else {
+      for (int off = 1; off < lanes; off <<= 1)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) m[j] = nan_max(__shfl_xor(m[j], off), m[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = lane + j * TPR, c = i * N;
+      const bool zero = m[j] < kTinyGroup;
+      const float inv = zero ? 0.f : kE4m3Max / m[j];
+      if (c < width) {
+        if (whole ? i == 0 : i % lanes == 0)
+          a.scales[whole ? row : row * (width / a.group) + c / a.group] = zero ? 0.f : m[j] / kE4m3Max;
+        uint8_t* q = a.q + at + c;
+        unsigned word[N / 4];
+#pragma unroll
+        for (int u = 0; u < N / 4; ++u) {
+          const float* v = &y[j][4 * u];
+          int p = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
+          word[u] = static_cast<unsigned>(__builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, p, true));
+        }
+        if (FULL || c + N <= width) {
+          struct __attribute__((packed, aligned(FULL ? N : 1))) Bytes {
+            unsigned w[N / 4];
+          };
+          Bytes b;
+#pragma unroll
+          for (int u = 0; u < N / 4; ++u) b.w[u] = word[u];
+          *reinterpret_cast<Bytes*>(q) = b;
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e)
+            if (c + e < width) q[e] = static_cast<uint8_t>(word[e / 4] >> (8 * (e % 4)));
+        }
+      }
+    }
+  }
+}
+
 template <class T>
 struct AddNormBwd {
   const T *h, *w, *dy, *dh;  // w, dh: may be null
@@ -139,6 +325,93 @@ __global__ __launch_bounds__(256) void add_norm_bwd_row_kernel(const AddNormBwd<
   if (threadIdx.x == 0 && a.s != nullptr) a.s[row] = s;
 }
 
+// The backward of rows in registers (as add_norm_kernel); the grid strides over the
+// rows and each thread keeps the weight gradient of its columns, so the partial
+// sums are one row a workgroup.
+template <class T, bool FULL, int TPR, int NV>
+__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void add_norm_bwd_kernel(const AddNormBwd<T> a) {
+  using V = NormVec<T>;
+  constexpr int N = V::N;
+  __shared__ float part[2][TPR / 64];
+  const int tid = threadIdx.x, lane = TPR == 64 ? tid & 63 : tid;
+  const int width = static_cast<int>(a.width);
+  const int64_t group = TPR == 64 ? static_cast<int64_t>(blockIdx.x) * 4 + (tid >> 6) : blockIdx.x;
+  const int64_t groups = static_cast<int64_t>(gridDim.x) * (TPR == 64 ? 4 : 1);
+  float dw[NV][N] = {};
+  typename V::type wv[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    wv[j] = a.w != nullptr ? norm_load<T, FULL>(a.w, lane + j * TPR, width) : typename V::type{};
+  for (int64_t row = group; row < a.rows; row += groups) {
+    const int64_t at = row * width;
+    typename V::type hv[NV], yv[NV], uv[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      hv[j] = norm_load<T, FULL>(a.h + at, lane + j * TPR, width);
+      yv[j] = norm_load<T, FULL>(a.dy + at, lane + j * TPR, width);
+    }
+    if (a.dh != nullptr) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) uv[j] = norm_load<T, FULL>(a.dh + at, lane + j * TPR, width);
+    }
+    float ss = 0.f, dot = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float h = to_float(static_cast<T>(hv[j][e]));
+        float g = to_float(static_cast<T>(yv[j][e]));
+        if (a.w != nullptr) g *= to_float(static_cast<T>(wv[j][e]));
+        ss += h * h;
+        dot += g * h;
+      }
+    ss = group_sum<64>(ss);
+    dot = group_sum<64>(dot);
+    if constexpr (TPR > 64) {
+      __syncthreads();  // the last row's sums have been read
+      if ((tid & 63) == 0) part[0][tid >> 6] = ss, part[1][tid >> 6] = dot;
+      __syncthreads();
+      ss = dot = 0.f;
+#pragma unroll
+      for (int u = 0; u < TPR / 64; ++u) ss += part[0][u], dot += part[1][u];
+    }
+    const float s = frsqrt(ss / static_cast<float>(width) + a.eps), back = s * s * (dot / static_cast<float>(width));
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      typename V::type o;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float h = to_float(static_cast<T>(hv[j][e])), dy = to_float(static_cast<T>(yv[j][e]));
+        const float g = a.w != nullptr ? dy * to_float(static_cast<T>(wv[j][e])) : dy;
+        float v = s * (g - h * back);
+        if (a.dh != nullptr) v += to_float(static_cast<T>(uv[j][e]));
+        o[e] = from_compute<T>(v);
+        dw[j][e] += dy * (h * s);
+      }
+      norm_store<T, FULL>(a.dx + at, lane + j * TPR, width, o);
+    }
+  }
+  if (a.dw == nullptr) return;
+  float* out = a.part + static_cast<int64_t>(blockIdx.x) * width;
+  if constexpr (TPR == 64) {  // the four waves' columns meet
+    __shared__ float meet[4][64 * NV * N];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < N; ++e) meet[tid >> 6][(lane + j * 64) * N + e] = dw[j][e];
+    __syncthreads();
+    for (int c = tid; c < width; c += 256) out[c] = (meet[0][c] + meet[1][c]) + (meet[2][c] + meet[3][c]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int c = (lane + j * TPR) * N + e;
+        if (c < width) out[c] = dw[j][e];
+      }
+  }
+}
+
 // Weight gradient of a chunk of rows, 64 columns a workgroup; then the chunks' sum.
 template <class T>
 __global__ __launch_bounds__(256) void add_norm_dw_kernel(const AddNormBwd<T> a) {
@@ -158,19 +431,25 @@ __global__ __launch_bounds__(256) void add_norm_dw_kernel(const AddNormBwd<T> a)
         (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
 }
 
+// The partial sums of 64 columns, sixteen waves each with every sixteenth part.
 template <class T>
-__global__ __launch_bounds__(256) void add_norm_dw_sum_kernel(const AddNormBwd<T> a, int64_t chunks) {
+__global__ __launch_bounds__(1024) void add_norm_dw_sum_kernel(const AddNormBwd<T> a, int64_t parts) {
   using C = typename NormCompute<T>::type;
-  __shared__ C part[4][64];
+  __shared__ C part[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
   C sum = C(0);
   if (c < a.width)
-    for (int64_t k = wave; k < chunks; k += 4) sum += a.part[k * a.width + c];
+#pragma unroll 4
+    for (int64_t k = wave; k < parts; k += 16) sum += a.part[k * a.width + c];
   part[wave][lane] = sum;
   __syncthreads();
-  if (wave == 0 && c < a.width)
-    a.dw[c] = from_compute<T>((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]));
+  if (wave == 0 && c < a.width) {
+    sum = part[0][lane];
+#pragma unroll
+    for (int u = 1; u < 16; ++u) sum += part[u][lane];
+    a.dw[c] = from_compute<T>(sum);
+  }
 }
 
 }  // namespace kda
@@ -181,8 +460,62 @@ using namespace kda;
 
 static bool grid_fits(int64_t n) { return n <= 0x7fffffffLL; }
 
+// The kernel for rows of `vectors` 16-byte vectors: a wave a row up to 256 of them,
+// a workgroup of 256 or 1024 threads up to 4096, wider rows (0) value by value.
+// With few rows the wave's four vectors go to four waves: latency.
+struct RowShape {
+  int threads, vectors;
+};
+static RowShape row_shape(int64_t width, int elem_bytes, int64_t rows) {
+  const int64_t n = (width * elem_bytes + 15) / 16;
+  if (elem_bytes == 8 || n > 4096) return {0, 0};
+  if (n <= 64) return {64, 1};
+  if (n <= 128) return {64, 2};
+  if (n <= 256) return rows >= 1024 ? RowShape{64, 4} : RowShape{256, 1};
+  if (n <= 512) return {256, 2};
+  if (n <= 1024) return {256, 4};
+  return n <= 2048 ? RowShape{1024, 2} : RowShape{1024, 4};
+}
+
+static bool whole_vectors(int64_t width, int elem_bytes, std::initializer_list<const void*> ptrs) {
+  uintptr_t bits = static_cast<uintptr_t>(width * elem_bytes);
+  for (const void* p : ptrs) bits |= reinterpret_cast<uintptr_t>(p);
+  return bits % 16 == 0;
+}
+
+template <class T, bool Q, bool FULL>
+static void launch_rows(const AddNorm<T>& a, RowShape r, hipStream_t s) {
+  const unsigned rows = static_cast<unsigned>(a.rows), waves = static_cast<unsigned>((a.rows + 3) / 4);
+  auto go = [&](auto kernel) {
+    const dim3 grid(r.threads == 64 ? waves : rows), block(r.threads == 64 ? 256 : r.threads);
+    hipLaunchKernelGGL(kernel, grid, block, 0, s, a);
+  };
+  if (r.threads == 64) {
+    if (r.vectors == 1) go(add_norm_kernel<T, Q, FULL, 64, 1>);
+    else if (r.vectors == 2) go(add_norm_kernel<T, Q, FULL, 64, 2>);
+    else go(add_norm_kernel<T, Q, FULL, 64, 4>);
+  } else if (r.threads == 256) {
+    if (r.vectors == 1) go(add_norm_kernel<T, Q, FULL, 256, 1>);
+    else if (r.vectors == 2) go(add_norm_kernel<T, Q, FULL, 256, 2>);
+    else go(add_norm_kernel<T, Q, FULL, 256, 4>);
+  } else {
+    if (r.vectors == 2) go(add_norm_kernel<T, Q, FULL, 1024, 2>);
+    else go(add_norm_kernel<T, Q, FULL, 1024, 4>);
+  }
+}
+
 template <class T, bool Q>
 static int run_add_norm(const AddNorm<T>& a, hipStream_t s) {
+  const RowShape r = row_shape(a.width, sizeof(T), a.rows);
+  if constexpr (sizeof(T) < 8) {
+    if (r.threads != 0) {
+      if (whole_vectors(a.width, sizeof(T), {a.x, a.r, a.w, a.h, a.y, a.q}))
+        launch_rows<T, Q, true>(a, r, s);
+      else
+        launch_rows<T, Q, false>(a, r, s);
+      return check_launch("add_norm");
+    }
+  }
   hipLaunchKernelGGL((add_norm_row_kernel<T, Q>), dim3(static_cast<unsigned>(a.rows)), dim3(256), 0, s, a);
   return check_launch("add_norm");
 }
@@ -214,15 +547,46 @@ int launch_add_norm(const void* x, const void* r, const void* w, void* h, void* 
   }
 }
 
-// Rows per chunk of the weight gradient's first pass: at most 64 chunks.
-static int64_t dw_chunk(int64_t rows) {
-  const int64_t n = (rows + 63) / 64;
-  return n < 16 ? 16 : n;
+// Partial weight gradients: one a workgroup of the strided backward, or of up to 64
+// chunks of rows.
+struct DwPlan {
+  int64_t parts, chunk;
+};
+static DwPlan dw_plan(int64_t rows, int64_t width, int elem_bytes) {
+  const RowShape r = row_shape(width, elem_bytes, rows);
+  if (r.threads != 0) {
+    const int64_t groups = r.threads == 64 ? (rows + 3) / 4 : rows, most = r.threads == 1024 ? 256 : 512;
+    return {groups < most ? groups : most, 0};
+  }
+  const int64_t n = (rows + 63) / 64, chunk = n < 16 ? 16 : n;
+  return {(rows + chunk - 1) / chunk, chunk};
 }
 
+static int elem_size(int dtype) { return dtype == KDA_DTYPE_F64 ? 8 : dtype == KDA_DTYPE_F32 ? 4 : 2; }
+
 size_t add_norm_bwd_workspace_bytes(int64_t rows, int64_t width, int dtype) {
-  const int64_t chunk = dw_chunk(rows), chunks = (rows + chunk - 1) / chunk;
-  return static_cast<size_t>(rows + chunks * width) * (dtype == KDA_DTYPE_F64 ? 8 : 4);
+  const DwPlan p = dw_plan(rows, width, elem_size(dtype));
+  const size_t c = dtype == KDA_DTYPE_F64 ? 8 : 4;
+  return (static_cast<size_t>(p.parts) * width + (p.chunk != 0 ? rows : 0)) * c;
+}
+
+template <class T, bool FULL>
+static void launch_bwd_rows(const AddNormBwd<T>& a, RowShape r, int64_t blocks, hipStream_t s) {
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(r.threads == 64 ? 256 : r.threads), 0, s, a);
+  };
+  if (r.threads == 64) {
+    if (r.vectors == 1) go(add_norm_bwd_kernel<T, FULL, 64, 1>);
+    else if (r.vectors == 2) go(add_norm_bwd_kernel<T, FULL, 64, 2>);
+    else go(add_norm_bwd_kernel<T, FULL, 64, 4>);
+  } else if (r.threads == 256) {
+    if (r.vectors == 1) go(add_norm_bwd_kernel<T, FULL, 256, 1>);
+    else if (r.vectors == 2) go(add_norm_bwd_kernel<T, FULL, 256, 2>);
+    else go(add_norm_bwd_kernel<T, FULL, 256, 4>);
+  } else {
+    if (r.vectors == 2) go(add_norm_bwd_kernel<T, FULL, 1024, 2>);
+    else go(add_norm_bwd_kernel<T, FULL, 1024, 4>);
+  }
 }
 
 template <class T>
@@ -232,15 +596,24 @@ static int add_norm_bwd_typed(const void* h, const void* w, const void* dy, cons
   AddNormBwd<T> a{};
   a.h = static_cast<const T*>(h), a.w = static_cast<const T*>(w), a.dy = static_cast<const T*>(dy);
   a.dh = static_cast<const T*>(dh), a.dx = static_cast<T*>(dx), a.dw = static_cast<T*>(dw);
-  a.rows = rows, a.width = width, a.eps = static_cast<typename NormCompute<T>::type>(eps), a.chunk = dw_chunk(rows);
-  if (dw != nullptr) a.s = static_cast<C*>(ws), a.part = a.s + rows;
-  hipLaunchKernelGGL((add_norm_bwd_row_kernel<T>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, s, a);
-  if (dw != nullptr) {
-    const unsigned blocks = static_cast<unsigned>((width + 63) / 64);
-    const int64_t chunks = (rows + a.chunk - 1) / a.chunk;
-    hipLaunchKernelGGL((add_norm_dw_kernel<T>), dim3(blocks, static_cast<unsigned>(chunks)), dim3(256), 0, s, a);
-    hipLaunchKernelGGL((add_norm_dw_sum_kernel<T>), dim3(blocks), dim3(256), 0, s, a, chunks);
+  a.rows = rows, a.width = width, a.eps = static_cast<C>(eps);
+  const RowShape r = row_shape(width, sizeof(T), rows);
+  const DwPlan p = dw_plan(rows, width, sizeof(T));
+  const unsigned columns = static_cast<unsigned>((width + 63) / 64);
+  a.part = static_cast<C*>(ws), a.chunk = p.chunk;
+  if (p.chunk != 0) {  // value by value
+    if (dw != nullptr) a.s = a.part + p.parts * width;
+    hipLaunchKernelGGL((add_norm_bwd_row_kernel<T>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, s, a);
+    if (dw != nullptr)
+      hipLaunchKernelGGL((add_norm_dw_kernel<T>), dim3(columns, static_cast<unsigned>(p.parts)), dim3(256), 0, s, a);
+  } else if constexpr (sizeof(T) < 8) {
+    if (whole_vectors(width, sizeof(T), {h, w, dy, dh, dx}))
+      launch_bwd_rows<T, true>(a, r, p.parts, s);
+    else
+      launch_bwd_rows<T, false>(a, r, p.parts, s);
   }
+  if (dw != nullptr)
+    hipLaunchKernelGGL((add_norm_dw_sum_kernel<T>), dim3(columns), dim3(1024), 0, s, a, p.parts);
   return check_launch("add_norm_bwd");
 }
 

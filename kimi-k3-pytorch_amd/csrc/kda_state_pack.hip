@@ -4,7 +4,8 @@
 // A state row (entry, head, key channel) of V values has a scale of its own:
 // the decay multiplies whole rows, so the rows of slow and fast channels differ
 // by orders of magnitude while the values of one row do not.
-//   scale = max|row| / 127,  q = round_half_even(row / scale),  read back: q scale
+//   scale = max|row| (1 / 127),  q = round_half_even(row / scale),  read back: q scale
+// with 1 / 127 rounded to f32 (the scale is off by two roundings, the quotient by none).
 // A row whose largest magnitude is under 2^-100 is held as zeros (its quotients
 // would leave f32), one with a value that is not finite has scale NaN.  The
 // other tensors of a cache (ShortConv histories, offsets) move as bytes.
@@ -39,7 +40,7 @@ struct MoveArgs {
 };
 static_assert(sizeof(MoveArgs) <= 4096, "the descriptors travel in the kernel argument block");
 
-// round_half_even(x / s) for |x| <= 127 s (1 + 2^-24), exactly: n is the whole
+// round_half_even(x / s) for |x| <= 127 s (1 + 2^-22), exactly: n is the whole
 // number nearest to the rounded product x (1 / s), one off at most; the
 // residual x - n s is exact in f32 (a multiple of half a step of s below its
 // half), so comparing it with s / 2 decides.
@@ -58,7 +59,7 @@ struct RowScale {
 __device__ __forceinline__ RowScale row_scale(float top) {
   if (!(top <= 3.402823466e38f)) return {__builtin_nanf(""), 0.f};
   if (top < kTinyRow) return {0.f, 0.f};
-  const float s = top / 127.f;
+  const float s = top * (1.f / 127.f);
   return {s, frcp(s)};
 }
 // the quotient, zeros for rows without a scale

@@ -232,7 +232,7 @@ def _one_device(tensors: Sequence[torch.Tensor]) -> torch.device:
 
 def pack_recurrent(state: torch.Tensor) -> PackedState:
     """Recurrent states ``[B,H,K,V]`` (f32, f16 or bf16) in 8 bits.  Every row
-    ``(b,h,k)`` of V values has its own scale, its largest magnitude over 127,
+    ``(b,h,k)`` of V values has its own scale, its largest magnitude times 1/127,
     and holds the nearest whole multiples of it (halves to even).  A row whose
     largest magnitude is under 2^-100 reads back as zeros, one with a value
     that is not finite as NaN.  No gradient: raises for a state that needs one."""

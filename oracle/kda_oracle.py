@@ -600,7 +600,7 @@ def pack_rows(state):
     amax = x.abs().amax(-1)
     finite = torch.isfinite(x).all(-1)
     zero = finite & (amax < 2.0 ** -100)
-    scales = torch.where(zero, torch.zeros_like(amax), amax / 127)
+    scales = torch.where(zero, torch.zeros_like(amax), amax * torch.tensor(1 / 127, dtype=torch.float32))
     use = finite & ~zero
     safe = torch.where(use, scales, torch.ones_like(scales)).double()
     values = torch.round(torch.where(use[..., None], x, torch.zeros_like(x)).double() / safe[..., None])
