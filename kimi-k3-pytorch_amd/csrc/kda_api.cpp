@@ -757,8 +757,8 @@ int kda_recurrent_fwd_packed(const void* q, const void* k, const void* v, const 
 
 static bool adapter_sizes(const kda_adapter_args* d) {
   const int64_t most = 0x7fffffffLL;
-  return d && d->rows > 0 && d->rows <= most && d->span > 0 && d->d_in > 0 && d->d_in <= 0xffffff && d->d_out > 0 &&
-         d->d_out <= 0xffffff && d->rank > 0 && d->rank <= 256 && d->adapters > 0 && d->adapters <= 0xffffff &&
+  return d && d->rows > 0 && d->rows <= most && d->span > 0 && d->d_in > 0 && d->d_in <= 0x7fffff && d->d_out > 0 &&
+         d->d_out <= 0x7fffff && d->rank > 0 && d->rank <= 256 && d->adapters > 0 && d->adapters <= 0xffffff &&
          (d->dtype == KDA_DTYPE_F32 || d->dtype == KDA_DTYPE_F16 || d->dtype == KDA_DTYPE_BF16);
 }
 
@@ -769,7 +769,7 @@ size_t kda_adapter_delta_workspace_bytes(const kda_adapter_args* args) {
 int kda_adapter_delta(const kda_adapter_args* args, void* stream) {
   g_detail[0] = '\0';
   if (!adapter_sizes(args)) {
-    set_detail("adapter_delta: positive sizes (widths and adapters below 2^24), rank up to 256, f32, f16 or bf16");
+    set_detail("adapter_delta: positive sizes (widths up to 2^23 - 1, adapters up to 2^24 - 1), rank up to 256, f32, f16 or bf16");
     return KDA_ERR_INVALID_ARGUMENT;
   }
   const kda_adapter_args& d = *args;
