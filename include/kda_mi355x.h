@@ -595,17 +595,22 @@ int kda_recurrent_fwd_packed(const void* q, const void* k, const void* v, const 
 
 /*
  * Low-rank adapters of many requests beside a shared projection, f32, f16 or bf16 tensors:
- *   y_m = bias + scaling_a b_a (a_a x_m),  a = ids[m / span]
- * in f32, rounded once: the projection's product x W^T is added by the caller (a GEMM with
- * beta = 1).  A row with a negative id gets the bias alone, one with an id >= adapters NaN.
+ *   y_m = x_m W^T + bias + scaling_a b_a (a_a x_m),  a = ids[m / span]
+ * in f32.  A row with a negative id has no adapter, one with an id >= adapters is NaN.
  *   x       : [rows, d_in];  y : [rows, d_out];  bias : [d_out] or NULL (zeros)
+ *   weight  : [d_out, d_in], or NULL: y without the product x W^T
  *   a       : [adapters, rank, d_in];  b : [adapters, d_out, rank]
  *   scaling : f32 [adapters] or NULL (1)
  *   ids     : int32 or int64 (ids_are_int64) [ceil(rows / span)], span >= 1 rows an id
- *   rank 1..256;  workspace of kda_adapter_delta_workspace_bytes(args), 16-byte aligned
+ *   rank 1..256;  workspace of kda_adapter_linear_workspace_bytes(args) (it may need none),
+ *   16-byte aligned
+ * The library forms the product itself for few rows (up to 32 with fewer than 16 rows an id,
+ * f16 or bf16, d_in a multiple of 64, x, weight and a 16-byte aligned); otherwise a call with
+ * a weight returns KDA_ERR_UNSUPPORTED (kda_adapter_linear_takes_weight says so beforehand): the
+ * caller leaves it out and adds the product by a GEMM with beta = 1.
  */
 typedef struct {
-  const void *x, *a, *b, *bias;
+  const void *x, *weight, *a, *b, *bias;
   const float* scaling;
   const void* ids;
   void* y;
@@ -615,9 +620,11 @@ typedef struct {
   int dtype, ids_are_int64;
 } kda_adapter_args;
 
-size_t kda_adapter_delta_workspace_bytes(const kda_adapter_args* args);
+int kda_adapter_linear_takes_weight(const kda_adapter_args* args);
 
-int kda_adapter_delta(const kda_adapter_args* args, void* stream);
+size_t kda_adapter_linear_workspace_bytes(const kda_adapter_args* args);
+
+int kda_adapter_linear(const kda_adapter_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -3,14 +3,18 @@
 // Row m's adapter is ids[m / span]: a negative id has none, an id past the stack
 // gives a row of NaN (the host cannot see it without waiting for the GPU).
 //
-// Two passes: s_m = A_a x_m in f32 (down), then c_a B_a s_m (up).  Rows that share
-// an adapter share its reading; whose rows they are is found by the kernels
+// First s_m = A_a x_m in f32 (down), then c_a B_a s_m (up).  Rows that share an
+// adapter share its reading; whose rows they are is found by the kernels
 // themselves, so a call needs no sorted batch and no plan:
-//  - long runs (a prompt's tokens): a workgroup owns 64 neighbouring rows and goes
-//    through the adapters it meets in them, mostly one;
-//  - few rows in any order (decode): the workgroup of row i counts the earlier rows
-//    with row i's adapter; where their number is a multiple of 16 it owns the next
-//    16 such rows, otherwise it has nothing to do.
+//  - runs (a prompt's tokens): a workgroup owns 32 neighbouring rows and goes through
+//    the adapters it meets in them, mostly one, both steps in one kernel; the
+//    shared projection is a library GEMM that adds to the result;
+//  - up to 512 rows in any order (decode): the workgroup of row i counts the earlier
+//    rows with row i's adapter; where their number is a multiple of 16 it owns
+//    the next 16 such rows, otherwise it has nothing to do.  A launch for each
+//    step; of up to 32 rows the projection is formed beside the first.
+#include <type_traits>
+
 #include "kda_launch.h"
 
 namespace kda {
@@ -37,21 +41,38 @@ __device__ __forceinline__ ad_f32x4 mma(Frag<float>::type a, Frag<float>::type b
   return c;
 }
 
-// Eight columns from k of a row of `len`; FULL: rows of whole vectors at aligned
-// addresses.  Columns past the row are zeros.
-template <class T, bool FULL>
-__device__ __forceinline__ typename Frag<T>::type load8(const T* row, int k, int len) {
+// EVEN calls: widths of whole 64-column slices, a rank of whole vectors and aligned
+// addresses, with code for nothing else: these kernels run for some ten
+// microseconds, and reading instructions that are skipped took a third of them.
+// Other calls load vectors at element alignment, which the hardware takes, and
+// the columns at a row's end one by one.
+
+// Eight columns, c to c + 7, of a row of `len`; zeros past it.
+template <class T, bool EVEN>
+__device__ __forceinline__ typename Frag<T>::type load8(const T* row, int c, int len) {
   typename Frag<T>::type v{};
-  if constexpr (FULL) {
-    if (k < len) v = *reinterpret_cast<const typename Frag<T>::type*>(row + k);
-  } else if (k + 8 <= len) {
-    v = *reinterpret_cast<const typename Frag<T>::loose*>(row + k);
+  if constexpr (EVEN) {
+    if (c < len) v = *reinterpret_cast<const typename Frag<T>::type*>(row + c);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (k + e < len) v[e] = row[k + e];
+    for (int e = 0; e < 8; ++e) {
+      const T x = row[c + e < len ? c + e : len - 1];
+      v[e] = c + e < len ? x : static_cast<T>(0.f);
+    }
   }
   return v;
+}
+
+// Sixteen columns from c of a row of `len`; zeros past it.
+template <class T, bool EVEN>
+__device__ __forceinline__ void load16(const T* row, int c, int len, typename Frag<T>::type (&v)[2]) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    if constexpr (EVEN)
+      v[u] = *reinterpret_cast<const typename Frag<T>::type*>(row + c + 8 * u);
+    else
+      v[u] = load8<T, false>(row, c + 8 * u, len);
+  }
 }
 
 template <class T>
@@ -61,12 +82,14 @@ struct Adapters {
   const void* ids;            // int32 or int64
   int ids64;
   int64_t rows;
-  int span, in, out, rank, n, splits;
-  T* y;      // [rows, out]
-  float* s;  // [splits, rows, rank]: sums over a part of the columns each
+  int span, in, out, rank, n, splits, parts;
+  T* y;         // [rows, out]
+  float* s;     // [splits, rows, rank]: sums over a part of the columns each
+  const T* weight;  // [out, in]
+  float* wide;  // [parts, rows, out]: x W^T, over a part of the columns each; parts 0 without
 };
 
-constexpr int kNone = -1, kMissing = -2;
+constexpr int kNone = -1, kMissing = -2, kNoRow = -3;
 
 // the row's adapter, kNone or kMissing
 template <class T>
@@ -80,265 +103,483 @@ __device__ __forceinline__ int below(uint64_t mask, int lane) {  // set bits und
   return __popcll(mask & ((uint64_t{1} << lane) - 1));
 }
 
-// ---- s = A x -------------------------------------------------------------------
-// A workgroup of four waves: 16 MT rows of one adapter, 16 NT of its rank, a part
-// of the columns, the waves every fourth 64-column slice of it; their sums meet
-// in LDS.  RUNS: 64 neighbouring rows, adapter by adapter.
-constexpr int kDownWaves = 4;
 constexpr int kAnyOrder = 512;  // rows in any order, at most
-constexpr int kSlice64 = 64;
 
-template <class T, bool FULL, int MT, int NT, bool RUNS>
-__global__ __launch_bounds__(64 * kDownWaves) void adapter_down_kernel(const Adapters<T> a) {
-  using v8 = typename Frag<T>::type;
-  constexpr int R = 16 * MT;
-  __shared__ int rowS[R];
-  __shared__ __attribute__((aligned(16))) float red[kDownWaves][NT * MT][256];
-  const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int j0 = blockIdx.z * 16 * NT;
-  const int slices = (a.in + kSlice64 - 1) / kSlice64, per = (slices + a.splits - 1) / a.splits;
-  const int first = blockIdx.y * per, last = first + per < slices ? first + per : slices;
-  float* s = a.s + static_cast<int64_t>(blockIdx.y) * a.rows * a.rank;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (RUNS ? R : 1);
-
-  int id, count;
-  uint64_t pending = 0;
-  int mine = kNone;  // RUNS: the adapter of the lane's row
-  if constexpr (RUNS) {
-    static_assert(R <= 64, "a lane per row");
-    if (lane < R && row0 + lane < a.rows) mine = adapter_of(a, row0 + lane);
-    pending = __ballot(mine >= 0);
-    if (pending == 0) return;
-  } else {
-    id = adapter_of(a, row0);
-    if (id < 0) return;
-    int of[kAnyOrder / 64];
+// The rows that the workgroup of `row` owns among the rows with its id, in rowS;
+// their number, none where an earlier row's workgroup owns it.
+template <int R, class T>
+__device__ __forceinline__ int gather_rows(const Adapters<T>& a, int row, int id, int* rowS) {
+  const int lane = threadIdx.x & 63;
+  int of[kAnyOrder / 64];
 #pragma unroll
-    for (int u = 0; u < kAnyOrder / 64; ++u) of[u] = 64 * u + lane < a.rows ? adapter_of(a, 64 * u + lane) : kNone;
-    const int self = static_cast<int>(row0);
-    int before = 0;
+  for (int u = 0; u < kAnyOrder / 64; ++u) of[u] = 64 * u + lane < a.rows ? adapter_of(a, 64 * u + lane) : kNoRow;
+  int before = 0;
 #pragma unroll
-    for (int u = 0; u < kAnyOrder / 64; ++u) before += __popcll(__ballot(of[u] == id && 64 * u + lane < self));
-    if (before % R != 0) return;
-    count = 0;
+  for (int u = 0; u < kAnyOrder / 64; ++u) before += __popcll(__ballot(of[u] == id && 64 * u + lane < row));
+  if (before % R != 0) return 0;  // the same in every wave
+  int count = 0;
 #pragma unroll
-    for (int u = 0; u < kAnyOrder / 64; ++u) {
-      const bool same = of[u] == id && 64 * u + lane >= self;
-      const uint64_t mask = __ballot(same);
-      const int at = count + below(mask, lane);
-      if (same && at < R && w == 0) rowS[at] = 64 * u + lane;
-      count += __popcll(mask);
-    }
-    count = count < R ? count : R;
-    __syncthreads();
+  for (int u = 0; u < kAnyOrder / 64; ++u) {
+    const bool same = of[u] == id && 64 * u + lane >= row;
+    const uint64_t mask = __ballot(same);
+    const int at = count + below(mask, lane);
+    if (same && at < R && threadIdx.x < 64) rowS[at] = 64 * u + lane;
+    count += __popcll(mask);
   }
-  do {
-    if constexpr (RUNS) {
-      id = __shfl(mine, __ffsll(static_cast<unsigned long long>(pending)) - 1);
-      const uint64_t mask = __ballot(mine == id);
-      pending &= ~mask;
-      count = __popcll(mask);
-      if (w == 0 && mine == id) rowS[below(mask, lane)] = static_cast<int>(row0) + lane;
-      __syncthreads();
-    }
-    const T *ap[NT], *xp[MT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {  // rows past the rank repeat its last one; their sums are dropped
-      const int j = j0 + 16 * t + li;
-      ap[t] = a.a + (static_cast<int64_t>(id) * a.rank + (j < a.rank ? j : a.rank - 1)) * a.in;
-    }
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const int r = 16 * t + li;
-      xp[t] = a.x + static_cast<int64_t>(rowS[r < count ? r : count - 1]) * a.in;
-    }
-    ad_f32x4 acc[NT][MT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int m = 0; m < MT; ++m) acc[t][m] = ad_f32x4{0.f, 0.f, 0.f, 0.f};
-    // E half slices in flight: of one slice with four row tiles, of two with one
-    constexpr int E = MT == 1 ? 4 : 2;
-    for (int c = first + w; c < last; c += kDownWaves * E / 2) {
-      v8 av[NT][E], xv[MT][E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int slice = c + kDownWaves * (e / 2);
-        const int k = slice < last ? slice * kSlice64 + 32 * (e & 1) + 8 * g : a.in;  // past the part: zeros
-#pragma unroll
-        for (int t = 0; t < NT; ++t) av[t][e] = load8<T, FULL>(ap[t], k, a.in);
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-          if (16 * m < count) xv[m][e] = load8<T, FULL>(xp[m], k, a.in);
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-        if (16 * m < count) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[t][m] = mma(av[t][e], xv[m][e], acc[t][m]);
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int m = 0; m < MT; ++m) *reinterpret_cast<ad_f32x4*>(&red[w][t * MT + m][4 * lane]) = acc[t][m];
-    __syncthreads();
-    for (int i = tid; i < NT * MT * 256; i += 64 * kDownWaves) {
-      const int jl = i % (16 * NT), rl = i / (16 * NT), j = j0 + jl;
-      const int at = 4 * ((rl & 15) + 16 * ((jl & 15) >> 2)) + (jl & 3), tile = (jl >> 4) * MT + (rl >> 4);
-      if (rl < count && j < a.rank) {
-        float sum = red[0][tile][at];
-#pragma unroll
-        for (int v = 1; v < kDownWaves; ++v) sum += red[v][tile][at];
-        s[static_cast<int64_t>(rowS[rl]) * a.rank + j] = sum;
-      }
-    }
-    if constexpr (RUNS) __syncthreads();  // before the next adapter's rows
-  } while (RUNS && pending != 0);
+  __syncthreads();
+  return count < R ? count : R;
 }
 
-// ---- y = bias + c B s, 64 neighbouring rows -----------------------------------
-// A workgroup of four waves: 64 rows, 64 columns a wave.  The sums s meet in LDS,
-// 64 of the rank at a time.  bf16: s as two bf16 values (2^-17 of it is left) on
-// bf16 products; f16 and f32: f32 products (f16 has not the range of s).
+// ---- matrix products of a workgroup ---------------------------------------------
+constexpr int kThreads = 512;
+constexpr int kWaves = kThreads / 64;
+constexpr int kSlice64 = 64;
+
+template <int TILES>
+struct Meet {  // partial tiles of the waves
+  __attribute__((aligned(16))) float red[kWaves / 2][TILES][256];
+};
+
+// The sum of the eight waves' 16 x 16 tiles, in two steps: the upper four waves'
+// tiles are added to the lower four's, which then meet.  `take(tile, n, m, sum)`
+// gets each element, row n and column m of its tile.
+template <int TILES, int ROOM, class F>
+__device__ __forceinline__ void meet_tiles(Meet<ROOM>& lds, ad_f32x4 (&acc)[TILES], F take) {
+  static_assert(TILES <= ROOM, "the tiles fit");
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  if (w >= kWaves / 2) {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) *reinterpret_cast<ad_f32x4*>(&lds.red[w - kWaves / 2][t][4 * lane]) = acc[t];
+  }
+  __syncthreads();
+  if (w < kWaves / 2) {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      ad_f32x4* p = reinterpret_cast<ad_f32x4*>(&lds.red[w][t][4 * lane]);
+      *p = *p + acc[t];
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < TILES * 256; i += kThreads) {
+    const int tile = i >> 8, n = i & 15, m = (i >> 4) & 15, at = 4 * (m + 16 * (n >> 2)) + (n & 3);
+    take(tile, n, m, (lds.red[0][tile][at] + lds.red[1][tile][at]) + (lds.red[2][tile][at] + lds.red[3][tile][at]));
+  }
+}
+
+// 16 NT rows of an adapter's A from row j0 times 16 MT rows of x (a lane's of each
+// tile at xp), over the slices first.. < last of 64 columns, the waves every
+// eighth of them, E half slices in flight.  acc[t * MT + m]: tile (t, m), this
+// wave's part.
+template <class T, bool EVEN, int MT, int NT, int E>
+__device__ __forceinline__ void down_product(const Adapters<T>& a, int id, int j0, const T* const (&xp)[MT], int first,
+                                             int last, ad_f32x4 (&acc)[NT * MT]) {
+  using v8 = typename Frag<T>::type;
+  using vec = typename std::conditional<EVEN, v8, typename Frag<T>::loose>::type;
+  const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const T* ap[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {  // rows past the rank repeat its last one; their sums are dropped
+    const int j = j0 + 16 * t + li;
+    ap[t] = a.a + (static_cast<int64_t>(id) * a.rank + (j < a.rank ? j : a.rank - 1)) * a.in;
+  }
+#pragma unroll
+  for (int t = 0; t < NT * MT; ++t) acc[t] = ad_f32x4{0.f, 0.f, 0.f, 0.f};
+  const int whole = EVEN || last * kSlice64 <= a.in ? last : last - 1;  // slices of 64 columns
+  for (int c = first + w; c < whole; c += kWaves * E / 2) {
+    v8 av[NT][E], xv[MT][E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int slice = c + kWaves * (e / 2);
+      const int k = (slice < whole ? slice : c) * kSlice64 + 32 * (e & 1) + 8 * g;  // past the part: read, not used
+#pragma unroll
+      for (int m = 0; m < MT; ++m) xv[m][e] = *reinterpret_cast<const vec*>(xp[m] + k);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) av[t][e] = *reinterpret_cast<const vec*>(ap[t] + k);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (c + kWaves * (e / 2) < whole) {  // uniform
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) acc[t * MT + m] = mma(av[t][e], xv[m][e], acc[t * MT + m]);
+      }
+  }
+  if (!EVEN && first < last && whole < last && (whole - first) % kWaves == w) {  // the slice that a row ends in
+#pragma unroll 1
+    for (int k = whole * kSlice64; k < a.in; k += 32) {
+      v8 av[NT], xv[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) xv[m] = load8<T, false>(xp[m], k + 8 * g, a.in);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) av[t] = load8<T, false>(ap[t], k + 8 * g, a.in);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t * MT + m] = mma(av[t], xv[m], acc[t * MT + m]);
+    }
+  }
+}
+
+// How B's products hold s.  bf16: as two bf16 values (2^-17 of it is left) on bf16
+// products; f16 and f32: f32 products (f16 has not the range of s).
 template <class T>
 struct UpType {
   using type = float;
+  static constexpr int P = 1;
 };
 template <>
 struct UpType<bf16> {
   using type = bf16;
+  static constexpr int P = 2;
 };
 
-constexpr int kUpRows = 64, kUpCols = 256, kUpRank = 64;
+template <class T, int R, int RANK>
+struct LowRows {  // s of R rows, RANK of the rank
+  using U = typename UpType<T>::type;
+  static constexpr int P = UpType<T>::P;
+  __attribute__((aligned(16))) U s[P][R][RANK + 8];
 
-template <class T>
-__global__ __launch_bounds__(256) void adapter_up_tile_kernel(const Adapters<T> a) {
+  __device__ __forceinline__ void put(int r, int j, float v) {
+    const U hi = static_cast<U>(v);
+    s[0][r][j] = hi;
+    if constexpr (P == 2) s[P - 1][r][j] = static_cast<U>(v - static_cast<float>(hi));
+  }
+};
+
+// What 64 columns from c0 need of B (the first 32 of the rank) and of the bias, for
+// a wave: asked for ahead of the sums they meet.  Row i of tile t is column
+// 16 (i / 4) + 4 t + i % 4, so a lane's results over the four tiles are sixteen
+// neighbouring columns of a row.
+template <class T, bool EVEN>
+struct UpLoads {
+  typename Frag<T>::type b[4];
+  typename Frag<T>::type bias[2];
+
+  __device__ __forceinline__ static const T* row(const Adapters<T>& a, int id, int c0, int t) {
+    const int li = threadIdx.x & 15, col = c0 + 16 * (li >> 2) + 4 * t + (li & 3);
+    return a.b + (static_cast<int64_t>(id) * a.out + (EVEN || col < a.out ? col : a.out - 1)) * a.rank;
+  }
+  __device__ __forceinline__ void ask(const Adapters<T>& a, int id, int c0) {
+    const int g = (threadIdx.x & 63) >> 4;
+    if (c0 >= a.out) return;
+    if (id >= 0) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) b[t] = load8<T, EVEN>(row(a, id, c0, t), 8 * g, a.rank);
+    }
+    bias[0] = bias[1] = typename Frag<T>::type{};
+    if (a.bias != nullptr) load16<T, EVEN>(a.bias, c0 + 16 * g, a.out, bias);
+  }
+};
+
+// y = bias + c B s (WIDE: + x W^T) of 64 columns from c0, a wave: s of 16 MT rows in
+// LDS.  rows[m]: the lane's row of tile m, or -1.
+template <class T, bool EVEN, bool WIDE, int MT, int R, int RANK>
+__device__ __forceinline__ void up_columns(const Adapters<T>& a, int id, float c, const UpLoads<T, EVEN>& in,
+                                           const LowRows<T, R, RANK>& low, const int (&rows)[MT], int c0) {
   using U = typename UpType<T>::type;
   using v8 = typename Frag<U>::type;
-  constexpr int P = sizeof(U) == 2 ? 2 : 1;  // parts of s
-  constexpr int LD = kUpRank + 8;
-  __shared__ __attribute__((aligned(16))) U sS[P][kUpRows][LD];
-  const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g = lane >> 4, w = tid >> 6;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kUpRows;
-  const int c0 = blockIdx.y * kUpCols + 64 * w;
-  int mine = kNone;  // adapter of row `lane`
-  if (row0 + lane < a.rows) mine = adapter_of(a, row0 + lane);
-  int of[4];  // adapters of the four rows the lane's results belong to
-#pragma unroll
-  for (int m = 0; m < 4; ++m) of[m] = __shfl(mine, 16 * m + li);
-  ad_f32x4 y[4][4];
+  constexpr int P = UpType<T>::P;
+  const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4, mycol = c0 + 16 * g;
+  ad_f32x4 d[4][MT];
 #pragma unroll
   for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      const float start = of[m] == kMissing ? __builtin_nanf("") : 0.f;
-      y[t][m] = ad_f32x4{start, start, start, start};
-    }
-  const uint64_t some = __ballot(mine >= 0);
-  for (int r0 = 0; some != 0 && r0 < a.rank; r0 += kUpRank) {
-    if (r0 != 0) __syncthreads();
-    for (int i = tid; i < kUpRows * kUpRank; i += 256) {
-      const int r = i / kUpRank, j = i % kUpRank;
-      float s = 0.f;
-      if (r0 + j < a.rank && row0 + r < a.rows) {
-        const float* p = a.s + (row0 + r) * a.rank + r0 + j;
-        for (int u = 0; u < a.splits; ++u) s += p[static_cast<int64_t>(u) * a.rows * a.rank];
+    for (int m = 0; m < MT; ++m) d[t][m] = ad_f32x4{0.f, 0.f, 0.f, 0.f};
+  if (id >= 0) {
+    typename Frag<T>::type raw[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) raw[t] = in.b[t];
+    for (int k = 0; k < a.rank; k += 32) {
+      if (k != 0) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) raw[t] = load8<T, EVEN>(UpLoads<T, EVEN>::row(a, id, c0, t), k + 8 * g, a.rank);
       }
-      const U hi = static_cast<U>(s);
-      sS[0][r][j] = hi;
-      if constexpr (P == 2) sS[1][r][j] = static_cast<U>(s - static_cast<float>(hi));
-    }
-    __syncthreads();
-    const int left = a.rank - r0 < kUpRank ? a.rank - r0 : kUpRank;
-    for (uint64_t pending = some; pending != 0;) {
-      const int id = __shfl(mine, __ffsll(static_cast<unsigned long long>(pending)) - 1);
-      pending &= ~__ballot(mine == id);
-      const float c = a.scaling != nullptr ? a.scaling[id] : 1.f;
-      const T* b = a.b + static_cast<int64_t>(id) * a.out * a.rank + r0;
+      v8 bv[4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int col = c0 + 16 * t + li;
-        const T* row = b + static_cast<int64_t>(col < a.out ? col : a.out - 1) * a.rank;
-        ad_f32x4 d[4];
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int m = 0; m < 4; ++m) d[m] = ad_f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int k = 0; k < left; k += 32) {
-          const auto raw = load8<T, false>(row, k + 8 * g, left);
-          v8 bv;
+        for (int e = 0; e < 8; ++e) bv[t][e] = static_cast<U>(raw[t][e]);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) bv[e] = static_cast<U>(raw[e]);
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int m = 0; m < 4; ++m)
+        for (int p = 0; p < P; ++p) {
+          const v8 sv = *reinterpret_cast<const v8*>(&low.s[p][16 * m + li][k + 8 * g]);
 #pragma unroll
-            for (int p = 0; p < P; ++p)
-              d[m] = mma(bv, *reinterpret_cast<const v8*>(&sS[p][16 * m + li][k + 8 * g]), d[m]);
+          for (int t = 0; t < 4; ++t) d[t][m] = mma(bv[t], sv, d[t][m]);
         }
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-          if (of[m] == id) y[t][m] += c * d[m];  // rows of other adapters: dropped, not weighted by zero
-      }
     }
   }
+  if (id == kMissing) c = __builtin_nanf("");  // times zero
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int col = c0 + 16 * t + 4 * g;
-    float bias[4];
+  for (int m = 0; m < MT; ++m) {
+    if (rows[m] < 0) continue;
+    const int64_t row = rows[m];
+    float y[16];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) bias[e] = a.bias != nullptr && col + e < a.out ? to_float(a.bias[col + e]) : 0.f;
+    for (int e = 0; e < 16; ++e)
+      y[e] = c * d[e >> 2][m][e & 3] + to_float(static_cast<T>(in.bias[e / 8][e % 8]));
+    if constexpr (WIDE) {
+      for (int u = 0; u < a.parts; ++u) {
+        Frag<float>::type part[2];
+        load16<float, EVEN>(a.wide + (u * a.rows + row) * a.out, mycol, a.out, part);
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      const int64_t row = row0 + 16 * m + li;
-      if (row >= a.rows) continue;
-      T* out = a.y + row * a.out + col;
-      typedef T o4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-      if (col + 4 <= a.out) {
-        o4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = from_compute<T>(y[t][m][e] + bias[e]);
-        *reinterpret_cast<o4*>(out) = v;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (col + e < a.out) out[e] = from_compute<T>(y[t][m][e] + bias[e]);
+        for (int e = 0; e < 16; ++e) y[e] += part[e / 8][e % 8];
       }
+    }
+    T* out = a.y + row * a.out + mycol;
+    constexpr int N = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(N), aligned(EVEN ? 16 : sizeof(T))));
+    if (EVEN || mycol + 16 <= a.out) {
+#pragma unroll
+      for (int u = 0; u < 16 / N; ++u) {
+        vec v;
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = from_compute<T>(y[u * N + e]);
+        *reinterpret_cast<vec*>(out + u * N) = v;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (mycol + e < a.out) out[e] = from_compute<T>(y[e]);
     }
   }
 }
 
-// ---- y = bias + c B s, a row a workgroup (few rows in any order) ----------------
-constexpr int kUpRowCols = 256;
+// All columns from c0 in steps, the next ones' loads ahead of the products (two
+// sets in turn: copying one to the other would wait for it).
+template <class T, bool EVEN, bool WIDE, int MT, int R, int RANK>
+__device__ __forceinline__ void up_all(const Adapters<T>& a, int id, float c, UpLoads<T, EVEN>& in,
+                                       const LowRows<T, R, RANK>& low, const int (&rows)[MT], int c0, int step) {
+  UpLoads<T, EVEN> next;
+  while (c0 < a.out) {
+    next.ask(a, id, c0 + step);
+    up_columns<T, EVEN, WIDE, MT>(a, id, c, in, low, rows, c0);
+    c0 += step;
+    if (c0 >= a.out) break;
+    in.ask(a, id, c0 + step);
+    up_columns<T, EVEN, WIDE, MT>(a, id, c, next, low, rows, c0);
+    c0 += step;
+  }
+}
 
 template <class T>
-__global__ __launch_bounds__(256) void adapter_up_row_kernel(const Adapters<T> a) {
-  __shared__ float sS[256];
-  const int64_t row = blockIdx.x;
-  const int id = adapter_of(a, row), col = blockIdx.y * kUpRowCols + threadIdx.x;
+__device__ __forceinline__ float factor(const Adapters<T>& a, int id) {
+  return id >= 0 && a.scaling != nullptr ? a.scaling[id] : 1.f;
+}
+
+// ---- runs of rows ---------------------------------------------------------------
+// y = bias + c B (A x) of 32 neighbouring rows a workgroup of eight waves, adapter
+// by adapter (every row's products are formed, the adapter's own rows are kept): s by 16 NT of the rank into LDS, then all columns, 64 a wave in
+// turn.  Two workgroups share the adapters of the rows where a run ends in them
+// (the second has nothing to do elsewhere).
+constexpr int kMaxRank = 256;
+constexpr int kRunTurns = 2;
+
+template <class T, bool EVEN, int NT>
+__global__ __launch_bounds__(kThreads) void adapter_run_kernel(const Adapters<T> a) {
+  constexpr int MT = 2, R = 16 * MT;
+  __shared__ Meet<2 * MT> meet;
+  __shared__ LowRows<T, R, kMaxRank> low;
+  const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, w = tid >> 6;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * R;
+  int mine = kNoRow;  // the adapter of the lane's row
+  if (lane < R && row0 + lane < a.rows) mine = adapter_of(a, row0 + lane);
+  const T* xp[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int64_t row = row0 + 16 * m + li;
+    xp[m] = a.x + (row < a.rows ? row : a.rows - 1) * a.in;
+  }
+  const int slices = (a.in + kSlice64 - 1) / kSlice64;
+  int turn = 0;
+  for (uint64_t pending = __ballot(mine != kNoRow); pending != 0;) {
+    const int id = __shfl(mine, __ffsll(static_cast<unsigned long long>(pending)) - 1);
+    pending &= ~__ballot(mine == id);
+    if (turn++ % gridDim.y != blockIdx.y) continue;  // another workgroup's; the same in every wave
+    int rows[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+      rows[m] = __shfl(mine, 16 * m + li) == id ? static_cast<int>(row0) + 16 * m + li : -1;
+    UpLoads<T, EVEN> first;
+    first.ask(a, id, 64 * w);
+    const float c = factor(a, id);
+    if (id >= 0) {
+      for (int j0 = 0; j0 < a.rank; j0 += 16 * NT) {
+        ad_f32x4 acc[NT * MT];
+        down_product<T, EVEN, MT, NT, NT == 1 ? 8 : 4>(a, id, j0, xp, 0, slices, acc);
+#pragma unroll
+        for (int t0 = 0; t0 < NT; t0 += 2) {  // two rank tiles at a time
+          constexpr int N = NT < 2 ? 1 : 2;
+          ad_f32x4 some[N * MT];
+#pragma unroll
+          for (int t = 0; t < N * MT; ++t) some[t] = acc[t0 * MT + t];
+          if (t0 != 0) __syncthreads();
+          meet_tiles<N * MT>(meet, some, [&](int tile, int n, int m, float sum) {
+            const int j = j0 + 16 * (t0 + tile / MT) + n;
+            if (j < kMaxRank) low.put(16 * (tile % MT) + m, j, j < a.rank ? sum : 0.f);
+            if (NT == 1) low.put(16 * (tile % MT) + m, j + 16, 0.f);  // products take 32 of the rank
+          });
+        }
+        __syncthreads();
+      }
+    }
+    up_all<T, EVEN, false, MT>(a, id, c, first, low, rows, 64 * w, 64 * kWaves);
+    __syncthreads();  // before the next adapter's sums
+  }
+}
+
+// ---- few rows in any order --------------------------------------------------------
+// s of 16 rows of one adapter, 16 NT of its rank, over a part of the columns.
+template <class T, bool EVEN, int NT>
+__device__ __forceinline__ void down_body(const Adapters<T>& a, int row, int part, int ranks, Meet<NT>& meet,
+                                          int* rowS) {
+  const int id = adapter_of(a, row);
+  if (id < 0) return;
+  const int count = gather_rows<16>(a, row, id, rowS);
+  if (count == 0) return;
+  const int slices = (a.in + kSlice64 - 1) / kSlice64, per = (slices + a.splits - 1) / a.splits;
+  const int first = part * per, last = first + per < slices ? first + per : slices;
+  float* s = a.s + static_cast<int64_t>(part) * a.rows * a.rank;
+  const int li = threadIdx.x & 15;
+  const T* xp[1] = {a.x + static_cast<int64_t>(rowS[li < count ? li : count - 1]) * a.in};
+  ad_f32x4 acc[NT];
+  down_product<T, EVEN, 1, NT, 4>(a, id, ranks * 16 * NT, xp, first, last, acc);
+  meet_tiles<NT>(meet, acc, [&](int tile, int n, int m, float sum) {
+    const int j = ranks * 16 * NT + 16 * tile + n;
+    if (m < count && j < a.rank) s[static_cast<int64_t>(rowS[m]) * a.rank + j] = sum;
+  });
+}
+
+template <class T, bool EVEN, int NT>
+__global__ __launch_bounds__(kThreads) void adapter_down_kernel(const Adapters<T> a) {
+  __shared__ Meet<NT> meet;
+  __shared__ int rowS[16];
+  down_body<T, EVEN, NT>(a, blockIdx.x, blockIdx.y, blockIdx.z, meet, rowS);
+}
+
+// x W^T of 16 NT weight rows and 16 MT rows of x over a part of the columns, in f32.
+template <class T, int MT, int NT>
+__device__ __forceinline__ void wide_body(const Adapters<T>& a, int block, Meet<NT * MT>& meet) {
+  using v8 = typename Frag<T>::type;
+  const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int across = (a.out + 16 * NT - 1) / (16 * NT);
+  const int n0 = (block % across) * 16 * NT, part = block / across;
+  const T *wp[NT], *xp[MT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {  // rows past the weight repeat its last one; their results are dropped
+    const int row = n0 + 16 * t + li;
+    wp[t] = a.weight + static_cast<int64_t>(row < a.out ? row : a.out - 1) * a.in + 8 * g;
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const int64_t row = 16 * t + li;
+    xp[t] = a.x + (row < a.rows ? row : a.rows - 1) * a.in + 8 * g;
+  }
+  ad_f32x4 acc[NT * MT];
+#pragma unroll
+  for (int t = 0; t < NT * MT; ++t) acc[t] = ad_f32x4{0.f, 0.f, 0.f, 0.f};
+  const int all = a.in / kSlice64, per = (all + a.parts - 1) / a.parts;
+  const int slices = part * per + per < all ? part * per + per : all;
+  constexpr int U = 4;  // slices in flight
+  for (int s0 = part * per + w; s0 < slices; s0 += kWaves * U) {
+    v8 wv[U][NT][2], xv[U][MT][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = s0 + u * kWaves;
+      const int k = (c < slices ? c : s0) * kSlice64;  // past the end: a slice already read, not used
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) wv[u][t][e] = *reinterpret_cast<const v8*>(wp[t] + k + 32 * e);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) xv[u][m][e] = *reinterpret_cast<const v8*>(xp[m] + k + 32 * e);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u * kWaves < slices) {  // uniform
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) acc[t * MT + m] = mma(wv[u][t][e], xv[u][m][e], acc[t * MT + m]);
+      }
+    }
+  }
+  meet_tiles<NT * MT>(meet, acc, [&](int tile, int n, int m, float sum) {
+    const int col = n0 + 16 * (tile / MT) + n, row = 16 * (tile % MT) + m;
+    if (col < a.out && row < a.rows) a.wide[(part * a.rows + row) * a.out + col] = sum;
+  });
+}
+
+// Both in one launch, for up to 16 MT rows: workgroups that form s and workgroups
+// that form x W^T.  Neither waits for the other, and the weights, whose bytes
+// bound the call, are read while s is formed.
+template <class T, bool EVEN, int MT>
+__global__ __launch_bounds__(kThreads) void adapter_both_kernel(const Adapters<T> a, int wide_blocks, int rank_blocks) {
+  constexpr int NT = 2;
+  __shared__ union {
+    Meet<NT * MT> wide;
+    struct {
+      Meet<NT> meet;
+      int rows[16];
+    } down;
+  } lds;
+  const int b = static_cast<int>(blockIdx.x);
+  if (b < wide_blocks) {
+    wide_body<T, MT, NT>(a, b, lds.wide);
+  } else {
+    const int d = b - wide_blocks, part = d % a.splits, ranks = d / a.splits % rank_blocks;
+    down_body<T, EVEN, NT>(a, d / a.splits / rank_blocks, part, ranks, lds.down.meet, lds.down.rows);
+  }
+}
+
+// y of 16 rows with one id (an adapter, none, or a missing one), the workgroup's four
+// waves 64 columns each in turn.
+template <class T, bool EVEN, bool WIDE>
+__global__ __launch_bounds__(256) void adapter_up_kernel(const Adapters<T> a) {
+  __shared__ LowRows<T, 16, kMaxRank> low;
+  __shared__ int rowS[16];
+  const int id = adapter_of(a, blockIdx.x), count = gather_rows<16>(a, blockIdx.x, id, rowS);
+  if (count == 0) return;
+  const int c0 = 64 * (4 * blockIdx.y + (threadIdx.x >> 6));
+  UpLoads<T, EVEN> first;
+  first.ask(a, id, c0);
+  const float c = factor(a, id);
   if (id >= 0) {
-    if (static_cast<int>(threadIdx.x) < a.rank) {
-      float s = 0.f;
-      for (int u = 0; u < a.splits; ++u) s += a.s[(u * a.rows + row) * a.rank + threadIdx.x];
-      sS[threadIdx.x] = s;
+    const int quads = (a.rank + 31) / 32 * 8;
+    for (int i = threadIdx.x; i < 16 * quads; i += 256) {
+      const int r = i / quads, j = i % quads * 4;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      if (r < count) {
+        const float* p = a.s + static_cast<int64_t>(rowS[r]) * a.rank + j;
+        for (int u = 0; u < a.splits; ++u, p += a.rows * a.rank) {
+          if constexpr (EVEN) {
+            if (j < a.rank) {
+              const ad_f32x4 v = *reinterpret_cast<const ad_f32x4*>(p);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sum[e] += v[e];
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (j + e < a.rank) sum[e] += p[e];
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) low.put(r, j + e, sum[e]);
     }
     __syncthreads();
   }
-  if (col >= a.out) return;
-  float y = id == kMissing ? __builtin_nanf("") : 0.f;
-  if (id >= 0) {
-    const T* b = a.b + (static_cast<int64_t>(id) * a.out + col) * a.rank;
-    for (int j = 0; j < a.rank; j += 8) {
-      const auto v = load8<T, false>(b, j, a.rank);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (j + e < a.rank) y += sS[j + e] * to_float(static_cast<T>(v[e]));
-    }
-    if (a.scaling != nullptr) y *= a.scaling[id];
-  }
-  if (a.bias != nullptr) y += to_float(a.bias[col]);
-  a.y[row * a.out + col] = from_compute<T>(y);
+  const int li = threadIdx.x & 15;
+  const int rows[1] = {li < count ? rowS[li] : -1};
+  up_all<T, EVEN, WIDE, 1>(a, id, c, first, low, rows, c0, 256 * gridDim.y);
 }
 
 }  // namespace kda
@@ -350,58 +591,104 @@ using namespace kda;
 // Few rows whose ids may lie in any order go by adapter, the rest by runs.
 static bool by_adapter(const kda_adapter_args& d) { return d.rows <= kAnyOrder && d.span < 16; }
 
-// Parts of the columns: of 512, so that a wave has two slices, up to eight parts
-// and, of runs, as many as make a thousand workgroups.
+// Parts of the columns of A x: of 1024, so that a wave has two slices, up to eight.
 static int column_splits(const kda_adapter_args& d) {
-  const int64_t n = (d.d_in + 511) / 512, tiles = (d.rows + 63) / 64;
-  const int64_t most = by_adapter(d) ? 8 : (1023 + tiles) / tiles < 8 ? (1023 + tiles) / tiles : 8;
-  return static_cast<int>(n < most ? n : most);
+  const int64_t n = (d.d_in + 1023) / 1024;
+  return static_cast<int>(n < 8 ? n : 8);
 }
 
-size_t adapter_delta_workspace_bytes(const kda_adapter_args& d) {
-  return static_cast<size_t>(column_splits(d)) * d.rows * d.rank * 4;
+// Parts of the columns of x W^T: four slices a wave at most (one round of loads),
+// and 256 workgroups where a wave keeps two slices.
+static int wide_parts(const kda_adapter_args& d) {
+  const int64_t slices = d.d_in / 64, across = (d.d_out + 31) / 32;
+  const int64_t fit = (slices + 31) / 32, fill = (255 + across) / across, most = slices / 16;
+  const int64_t n = fill < most ? fill : most;
+  return static_cast<int>(n > fit ? n : fit);
 }
 
-template <class T, bool FULL, int MT, bool RUNS>
-static void launch_down(const Adapters<T>& a, int64_t blocks, hipStream_t s) {
-  auto go = [&](auto kernel, int ranks) {
-    const dim3 grid(static_cast<unsigned>(blocks), a.splits, static_cast<unsigned>((a.rank + ranks - 1) / ranks));
-    hipLaunchKernelGGL(kernel, grid, dim3(64 * kDownWaves), 0, s, a);
-  };
+// The projection of few rows beside the adapters, in this library's own kernel.
+bool adapter_takes_projection(const kda_adapter_args& d) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(d.x) | reinterpret_cast<uintptr_t>(d.a) |
+                         reinterpret_cast<uintptr_t>(d.weight);
+  return d.dtype != KDA_DTYPE_F32 && by_adapter(d) && d.rows <= 32 && d.d_in % 64 == 0 && bits % 16 == 0;
+}
+
+static int64_t s_floats(const kda_adapter_args& d) {
+  return by_adapter(d) ? (static_cast<int64_t>(column_splits(d)) * d.rows * d.rank + 7) / 8 * 8 : 0;
+}
+
+size_t adapter_workspace_bytes(const kda_adapter_args& d) {
+  const int64_t wide = d.weight != nullptr ? wide_parts(d) * d.rows * d.d_out : 0;
+  return static_cast<size_t>(s_floats(d) + wide) * 4;
+}
+
+template <class T>
+static Adapters<T> adapters_of(const kda_adapter_args& d) {
+  Adapters<T> a{};
+  a.x = static_cast<const T*>(d.x), a.a = static_cast<const T*>(d.a), a.b = static_cast<const T*>(d.b);
+  a.bias = static_cast<const T*>(d.bias), a.scaling = d.scaling, a.ids = d.ids, a.ids64 = d.ids_are_int64;
+  a.span = static_cast<int>(d.span < d.rows ? d.span : d.rows), a.rows = d.rows;
+  a.in = static_cast<int>(d.d_in), a.out = static_cast<int>(d.d_out);
+  a.rank = static_cast<int>(d.rank), a.n = static_cast<int>(d.adapters), a.splits = column_splits(d);
+  a.y = static_cast<T*>(d.y), a.s = static_cast<float*>(d.workspace);
+  return a;
+}
+
+static bool even_call(const kda_adapter_args& d) {
+  const void* ptrs[] = {d.x, d.a, d.b, d.y, d.bias};
+  uintptr_t bits = 0;
+  for (const void* p : ptrs) bits |= reinterpret_cast<uintptr_t>(p);
+  const int vector = d.dtype == KDA_DTYPE_F32 ? 32 : 16;
+  return d.d_in % kSlice64 == 0 && d.d_out % 64 == 0 && d.rank % 8 == 0 && bits % vector == 0;
+}
+
+// Workgroups along the columns: about a thousand in all, whose rows are found once.
+template <class T, bool EVEN, bool WIDE>
+static void launch_up(const Adapters<T>& a, hipStream_t s) {
+  const int64_t blocks = (a.out + 255) / 256, fill = (1023 + a.rows) / a.rows;
+  hipLaunchKernelGGL((adapter_up_kernel<T, EVEN, WIDE>),
+                     dim3(static_cast<unsigned>(a.rows), static_cast<unsigned>(blocks < fill ? blocks : fill)), dim3(256),
+                     0, s, a);
+}
+
+template <class T, bool EVEN>
+static void launch_delta(const Adapters<T>& a, bool any_order, hipStream_t s) {
+  if (!any_order) {
+    const dim3 grid(static_cast<unsigned>((a.rows + 31) / 32), kRunTurns);
+    if (a.rank <= 16)
+      hipLaunchKernelGGL((adapter_run_kernel<T, EVEN, 1>), grid, dim3(kThreads), 0, s, a);
+    else if (a.rank <= 32)
+      hipLaunchKernelGGL((adapter_run_kernel<T, EVEN, 2>), grid, dim3(kThreads), 0, s, a);
+    else
+      hipLaunchKernelGGL((adapter_run_kernel<T, EVEN, 4>), grid, dim3(kThreads), 0, s, a);
+    return;
+  }
+  const dim3 grid(static_cast<unsigned>(a.rows), a.splits, static_cast<unsigned>((a.rank + 31) / 32));
   if (a.rank <= 16)
-    go(adapter_down_kernel<T, FULL, MT, 1, RUNS>, 16);
+    hipLaunchKernelGGL((adapter_down_kernel<T, EVEN, 1>), grid, dim3(kThreads), 0, s, a);
   else
-    go(adapter_down_kernel<T, FULL, MT, 2, RUNS>, 32);
+    hipLaunchKernelGGL((adapter_down_kernel<T, EVEN, 2>), grid, dim3(kThreads), 0, s, a);
+  launch_up<T, EVEN, false>(a, s);
+}
+
+template <class T, bool EVEN>
+static void launch_both(const Adapters<T>& a, hipStream_t s) {
+  const int wide = a.parts * ((a.out + 31) / 32), ranks = (a.rank + 31) / 32;  // 2^30 workgroups at most
+  const dim3 grid(static_cast<unsigned>(wide + a.rows * a.splits * ranks));
+  if (a.rows <= 16)
+    hipLaunchKernelGGL((adapter_both_kernel<T, EVEN, 1>), grid, dim3(kThreads), 0, s, a, wide, ranks);
+  else
+    hipLaunchKernelGGL((adapter_both_kernel<T, EVEN, 2>), grid, dim3(kThreads), 0, s, a, wide, ranks);
+  launch_up<T, EVEN, true>(a, s);
 }
 
 template <class T>
 static int run_adapter_delta(const kda_adapter_args& d, hipStream_t s) {
-  Adapters<T> a{};
-  a.x = static_cast<const T*>(d.x), a.a = static_cast<const T*>(d.a), a.b = static_cast<const T*>(d.b);
-  a.bias = static_cast<const T*>(d.bias), a.scaling = d.scaling, a.ids = d.ids, a.ids64 = d.ids_are_int64;
-  a.span = static_cast<int>(d.span < d.rows ? d.span : d.rows), a.rows = d.rows, a.in = static_cast<int>(d.d_in), a.out = static_cast<int>(d.d_out);
-  a.rank = static_cast<int>(d.rank), a.n = static_cast<int>(d.adapters), a.splits = column_splits(d);
-  a.y = static_cast<T*>(d.y), a.s = static_cast<float*>(d.workspace);
-  const bool full = d.d_in % 8 == 0 &&
-                    (reinterpret_cast<uintptr_t>(d.x) | reinterpret_cast<uintptr_t>(d.a)) % (8 * sizeof(T)) == 0;
-  if (by_adapter(d)) {
-    if (full)
-      launch_down<T, true, 1, false>(a, a.rows, s);
-    else
-      launch_down<T, false, 1, false>(a, a.rows, s);
-    hipLaunchKernelGGL((adapter_up_row_kernel<T>),
-                       dim3(static_cast<unsigned>(a.rows), static_cast<unsigned>((a.out + kUpRowCols - 1) / kUpRowCols)),
-                       dim3(256), 0, s, a);
-  } else {
-    const int64_t tiles = (a.rows + 63) / 64;
-    if (full)
-      launch_down<T, true, 4, true>(a, tiles, s);
-    else
-      launch_down<T, false, 4, true>(a, tiles, s);
-    hipLaunchKernelGGL((adapter_up_tile_kernel<T>),
-                       dim3(static_cast<unsigned>(tiles), static_cast<unsigned>((a.out + kUpCols - 1) / kUpCols)),
-                       dim3(256), 0, s, a);
-  }
+  const Adapters<T> a = adapters_of<T>(d);
+  if (even_call(d))
+    launch_delta<T, true>(a, by_adapter(d), s);
+  else
+    launch_delta<T, false>(a, by_adapter(d), s);
   return check_launch("adapter_delta");
 }
 
@@ -411,6 +698,21 @@ int launch_adapter_delta(const kda_adapter_args& d, hipStream_t s) {
     case KDA_DTYPE_F16: return run_adapter_delta<f16>(d, s);
     default: return run_adapter_delta<float>(d, s);
   }
+}
+
+template <class T>
+static int run_adapter_linear(const kda_adapter_args& d, hipStream_t s) {
+  Adapters<T> a = adapters_of<T>(d);
+  a.weight = static_cast<const T*>(d.weight), a.wide = a.s + s_floats(d), a.parts = wide_parts(d);
+  if (even_call(d))
+    launch_both<T, true>(a, s);
+  else
+    launch_both<T, false>(a, s);
+  return check_launch("adapter_linear");
+}
+
+int launch_adapter_linear(const kda_adapter_args& d, hipStream_t s) {
+  return d.dtype == KDA_DTYPE_BF16 ? run_adapter_linear<bf16>(d, s) : run_adapter_linear<f16>(d, s);
 }
 
 }  // namespace kda_host

@@ -762,31 +762,42 @@ static bool adapter_sizes(const kda_adapter_args* d) {
          (d->dtype == KDA_DTYPE_F32 || d->dtype == KDA_DTYPE_F16 || d->dtype == KDA_DTYPE_BF16);
 }
 
-size_t kda_adapter_delta_workspace_bytes(const kda_adapter_args* args) {
-  return adapter_sizes(args) ? adapter_delta_workspace_bytes(*args) : 0;
+int kda_adapter_linear_takes_weight(const kda_adapter_args* args) {
+  return adapter_sizes(args) && adapter_takes_projection(*args) ? 1 : 0;
 }
 
-int kda_adapter_delta(const kda_adapter_args* args, void* stream) {
+size_t kda_adapter_linear_workspace_bytes(const kda_adapter_args* args) {
+  return adapter_sizes(args) ? adapter_workspace_bytes(*args) : 0;
+}
+
+int kda_adapter_linear(const kda_adapter_args* args, void* stream) {
   g_detail[0] = '\0';
   if (!adapter_sizes(args)) {
-    set_detail("adapter_delta: positive sizes (widths up to 2^23 - 1, adapters up to 2^24 - 1), rank up to 256, f32, f16 or bf16");
+    set_detail("adapter_linear: positive sizes (widths up to 2^23 - 1, adapters up to 2^24 - 1), rank up to 256, "
+               "f32, f16 or bf16");
     return KDA_ERR_INVALID_ARGUMENT;
   }
   const kda_adapter_args& d = *args;
   if (!d.x || !d.a || !d.b || !d.ids || !d.y) {
-    set_detail("adapter_delta: x, a, b, ids and y must be non-null");
+    set_detail("adapter_linear: x, a, b, ids and y must be non-null");
     return KDA_ERR_INVALID_ARGUMENT;
   }
-  const size_t need = adapter_delta_workspace_bytes(d);
-  if (!d.workspace || d.workspace_bytes < need) {
-    set_detail("adapter_delta: workspace of %zu bytes needed", need);
+  if (d.weight && !adapter_takes_projection(d)) {
+    set_detail("adapter_linear: the product with the weight is formed here for up to 32 f16 or bf16 rows of whole, "
+               "aligned 64-column slices with fewer than 16 rows an id");
+    return KDA_ERR_UNSUPPORTED;
+  }
+  const size_t need = adapter_workspace_bytes(d);
+  if (need > 0 && (!d.workspace || d.workspace_bytes < need)) {
+    set_detail("adapter_linear: workspace of %zu bytes needed", need);
     return KDA_ERR_WORKSPACE;
   }
   if (reinterpret_cast<uintptr_t>(d.workspace) % 16 != 0) {
-    set_detail("adapter_delta: the workspace must be 16-byte aligned");
+    set_detail("adapter_linear: the workspace must be 16-byte aligned");
     return KDA_ERR_INVALID_ARGUMENT;
   }
-  return launch_adapter_delta(d, static_cast<hipStream_t>(stream));
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  return d.weight ? launch_adapter_linear(d, s) : launch_adapter_delta(d, s);
 }
 
 }  // extern "C"

@@ -184,8 +184,12 @@ int launch_recurrent_packed(const void* q, const void* k, const void* v, const v
                             int64_t V, hipStream_t stream);
 
 // Adapters of many requests beside a shared projection (csrc/kda_adapter.hip).
-size_t adapter_delta_workspace_bytes(const kda_adapter_args& d);
+bool adapter_takes_projection(const kda_adapter_args& d);
+
+size_t adapter_workspace_bytes(const kda_adapter_args& d);
 
 int launch_adapter_delta(const kda_adapter_args& d, hipStream_t stream);
+
+int launch_adapter_linear(const kda_adapter_args& d, hipStream_t stream);
 
 }  // namespace kda_host

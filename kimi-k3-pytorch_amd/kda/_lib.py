@@ -55,7 +55,8 @@ class AdapterArgs(ctypes.Structure):
     """kda_adapter_args, field for field."""
 
     _fields_ = (
-        [(name, ctypes.c_void_p) for name in ("x", "a", "b", "bias", "scaling", "ids", "y", "workspace")]
+        [(name, ctypes.c_void_p) for name in ("x", "weight", "a", "b", "bias", "scaling", "ids", "y",
+                                                 "workspace")]
         + [("workspace_bytes", ctypes.c_size_t)]
         + [(name, ctypes.c_int64) for name in ("rows", "span", "d_in", "d_out", "rank", "adapters")]
         + [("dtype", ctypes.c_int), ("ids_are_int64", ctypes.c_int)]
@@ -136,8 +137,9 @@ SIGNATURES = {
     "kda_layer_decode": (_I, [_P, _P]),
     "kda_state_move": (_I, [_P, _I, _I, _P, _L, _P, _L, _L, _P, _P]),
     "kda_recurrent_fwd_packed": (_I, [_P] * 5 + [_I, _P, _P, _P, _L, _P, _P, _P, _L, _P] + [_L] * 5 + [_P]),
-    "kda_adapter_delta_workspace_bytes": (_S, [_P]),
-    "kda_adapter_delta": (_I, [_P, _P]),
+    "kda_adapter_linear_takes_weight": (_I, [_P]),
+    "kda_adapter_linear_workspace_bytes": (_S, [_P]),
+    "kda_adapter_linear": (_I, [_P, _P]),
     "kda_add_rmsnorm_fwd": (_I, [_P] * 5 + [_L, _L, ctypes.c_double, _I, _P]),
     "kda_add_rmsnorm_quant": (_I, [_P] * 6 + [_L, _L, _L, ctypes.c_double, _I, _P]),
     "kda_add_rmsnorm_bwd_workspace_bytes": (_S, [_L, _L, _I]),

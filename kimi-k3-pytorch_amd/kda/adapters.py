@@ -101,27 +101,32 @@ def adapter_linear(
     each request, ``[B]``, or of each token, ``[B,T]`` (packed documents):
     ``stack.a[id]`` and ``stack.b[id]``; a negative id has none.  The call does not
     wait for the GPU, so an id past the stack cannot raise: its rows are NaN.
-    f32 accumulation, the adapter's part rounded to the dtype before the
-    projection's product is added to it."""
+    f32 accumulation; few rows (decode) are rounded once, of many the adapter's part
+    is rounded to the dtype before the projection's product is added to it."""
     span = _check(x, weight, bias, stack, adapter_ids)
     d_in, (d_out, rows) = x.shape[-1], (weight.shape[0], x.shape[:-1].numel())
     y = torch.empty(*x.shape[:-1], d_out, dtype=x.dtype, device=x.device)
     if rows == 0:
         return y
-    xc, a, b, ids = (t.contiguous() for t in (x, stack.a, stack.b, adapter_ids))
+    xc, a, b, ids = x.contiguous(), stack.a.contiguous(), stack.b.contiguous(), adapter_ids.contiguous()
     bias = None if bias is None else bias.contiguous()
     scaling = None if stack.scaling is None else stack.scaling.contiguous()
     lib = _lib.load()
-    args = _lib.AdapterArgs(xc.data_ptr(), a.data_ptr(), b.data_ptr(), _lib.ptr(bias), _lib.ptr(scaling),
+    args = _lib.AdapterArgs(xc.data_ptr(), None, a.data_ptr(), b.data_ptr(), _lib.ptr(bias), _lib.ptr(scaling),
                             ids.data_ptr(), y.data_ptr(), None, 0, rows, span, d_in, d_out, a.shape[1], a.shape[0],
                             _lib.dtype_code(x.dtype), 1 if ids.dtype == torch.int64 else 0)
     ref = ctypes.addressof(args)
+    if weight.is_contiguous():
+        args.weight = weight.data_ptr()
+        if not lib.kda_adapter_linear_takes_weight(ref):
+            args.weight = None
     with _prep.on_device(x.device):
-        args.workspace_bytes = lib.kda_adapter_delta_workspace_bytes(ref)
+        args.workspace_bytes = lib.kda_adapter_linear_workspace_bytes(ref)
         workspace = _prep.workspace(args.workspace_bytes, x.device, "adapter_linear")
         args.workspace = _lib.ptr(workspace)
-        _lib.check(lib.kda_adapter_delta(ref, _prep.stream(x.device)))
-        y.view(rows, d_out).addmm_(xc.view(rows, d_in), weight.t())
+        _lib.check(lib.kda_adapter_linear(ref, _prep.stream(x.device)))
+        if args.weight is None:
+            y.view(rows, d_out).addmm_(xc.view(rows, d_in), weight.t())
     return y
 
 

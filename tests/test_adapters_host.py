@@ -70,22 +70,35 @@ def test_entry_point_rejects_bad_arguments():
     lib, p = _lib.load(), 4096
 
     def args(**kw):
-        fields = dict(x=p, a=p, b=p, bias=None, scaling=None, ids=p, y=p, workspace=p, workspace_bytes=1 << 30, rows=4,
+        fields = dict(x=p, weight=None, a=p, b=p, bias=None, scaling=None, ids=p, y=p, workspace=p, workspace_bytes=1 << 30, rows=4,
                       span=1, d_in=8, d_out=8, rank=4, adapters=2, dtype=2, ids_are_int64=1)
         return _lib.AdapterArgs(**{**fields, **kw})
 
     def call(**kw):
         d = args(**kw)
-        return lib.kda_adapter_delta(ctypes.addressof(d), None)
+        return lib.kda_adapter_linear(ctypes.addressof(d), None)
 
     for kw in (dict(x=None), dict(a=None), dict(b=None), dict(ids=None), dict(y=None), dict(rows=0), dict(span=0),
                dict(rows=1 << 31), dict(d_in=0), dict(d_in=1 << 24), dict(d_out=0), dict(rank=0), dict(rank=257),
                dict(adapters=0), dict(dtype=3), dict(workspace=p + 4)):
         assert call(**kw) == _lib.KDA_ERR_INVALID_ARGUMENT, kw
-    assert lib.kda_adapter_delta(None, None) == _lib.KDA_ERR_INVALID_ARGUMENT
+    assert lib.kda_adapter_linear(None, None) == _lib.KDA_ERR_INVALID_ARGUMENT
     d = args()
-    need = lib.kda_adapter_delta_workspace_bytes(ctypes.addressof(d))
+    need = lib.kda_adapter_linear_workspace_bytes(ctypes.addressof(d))
     assert need > 0
     assert call(workspace=None) == _lib.KDA_ERR_WORKSPACE and call(workspace_bytes=need - 1) == _lib.KDA_ERR_WORKSPACE
+    # the product with the weight: for few aligned 16-bit rows
+    few = dict(weight=p, d_in=64, rows=20)
+
+    def takes(**kw):
+        d = args(**{**few, **kw})  # lives as long as its address is used
+        return lib.kda_adapter_linear_takes_weight(ctypes.addressof(d))
+
+    assert takes() == 1 and takes(rows=32) == 1 and takes(dtype=1) == 1 and takes(span=15) == 1
+    for kw in (dict(rows=33), dict(dtype=0), dict(span=16), dict(d_in=96), dict(x=p + 8), dict(weight=p + 2), dict(a=p + 4)):
+        assert takes(**kw) == 0 and call(**{**few, **kw}) == _lib.KDA_ERR_UNSUPPORTED, kw
+    d, plain = args(**few), args(**{**few, "weight": None})
+    assert lib.kda_adapter_linear_workspace_bytes(ctypes.addressof(d)) > \
+        lib.kda_adapter_linear_workspace_bytes(ctypes.addressof(plain))
     d = args(rank=300)
-    assert lib.kda_adapter_delta_workspace_bytes(ctypes.addressof(d)) == 0
+    assert lib.kda_adapter_linear_workspace_bytes(ctypes.addressof(d)) == 0
