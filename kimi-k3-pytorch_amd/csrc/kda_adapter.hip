@@ -112,7 +112,10 @@ __device__ __forceinline__ int gather_rows(const Adapters<T>& a, int row, int id
   const int lane = threadIdx.x & 63;
   int of[kAnyOrder / 64];
 #pragma unroll
-  for (int u = 0; u < kAnyOrder / 64; ++u) of[u] = 64 * u + lane < a.rows ? adapter_of(a, 64 * u + lane) : kNoRow;
+  for (int u = 0; u < kAnyOrder / 64; ++u) {
+    of[u] = kNoRow;
+    if (64 * u < a.rows && 64 * u + lane < a.rows) of[u] = adapter_of(a, 64 * u + lane);
+  }
   int before = 0;
 #pragma unroll
   for (int u = 0; u < kAnyOrder / 64; ++u) before += __popcll(__ballot(of[u] == id && 64 * u + lane < row));
@@ -370,16 +373,16 @@ __device__ __forceinline__ float factor(const Adapters<T>& a, int id) {
 }
 
 // ---- runs of rows ---------------------------------------------------------------
-// y = bias + c B (A x) of 32 neighbouring rows a workgroup of eight waves, adapter
+// y = bias + c B (A x) of 16 MT neighbouring rows a workgroup of eight waves, adapter
 // by adapter (every row's products are formed, the adapter's own rows are kept): s by 16 NT of the rank into LDS, then all columns, 64 a wave in
 // turn.  Two workgroups share the adapters of the rows where a run ends in them
 // (the second has nothing to do elsewhere).
 constexpr int kMaxRank = 256;
 constexpr int kRunTurns = 2;
 
-template <class T, bool EVEN, int NT>
+template <class T, bool EVEN, int MT, int NT>
 __global__ __launch_bounds__(kThreads) void adapter_run_kernel(const Adapters<T> a) {
-  constexpr int MT = 2, R = 16 * MT;
+  constexpr int R = 16 * MT;
   __shared__ Meet<2 * MT> meet;
   __shared__ LowRows<T, R, kMaxRank> low;
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, w = tid >> 6;
@@ -431,9 +434,10 @@ __global__ __launch_bounds__(kThreads) void adapter_run_kernel(const Adapters<T>
 }
 
 // ---- few rows in any order --------------------------------------------------------
-// s of 16 rows of one adapter, 16 NT of its rank, over a part of the columns.
+// s of 16 rows of one adapter over a part of the columns: 16 NT of the rank from
+// block `ranks` on, every `step`th of them.
 template <class T, bool EVEN, int NT>
-__device__ __forceinline__ void down_body(const Adapters<T>& a, int row, int part, int ranks, Meet<NT>& meet,
+__device__ __forceinline__ void down_body(const Adapters<T>& a, int row, int part, int ranks, int step, Meet<NT>& meet,
                                           int* rowS) {
   const int id = adapter_of(a, row);
   if (id < 0) return;
@@ -444,19 +448,22 @@ __device__ __forceinline__ void down_body(const Adapters<T>& a, int row, int par
   float* s = a.s + static_cast<int64_t>(part) * a.rows * a.rank;
   const int li = threadIdx.x & 15;
   const T* xp[1] = {a.x + static_cast<int64_t>(rowS[li < count ? li : count - 1]) * a.in};
-  ad_f32x4 acc[NT];
-  down_product<T, EVEN, 1, NT, 4>(a, id, ranks * 16 * NT, xp, first, last, acc);
-  meet_tiles<NT>(meet, acc, [&](int tile, int n, int m, float sum) {
-    const int j = ranks * 16 * NT + 16 * tile + n;
-    if (m < count && j < a.rank) s[static_cast<int64_t>(rowS[m]) * a.rank + j] = sum;
-  });
+  for (int j0 = 16 * NT * ranks; j0 < a.rank; j0 += 16 * NT * step) {
+    ad_f32x4 acc[NT];
+    down_product<T, EVEN, 1, NT, 4>(a, id, j0, xp, first, last, acc);
+    meet_tiles<NT>(meet, acc, [&](int tile, int n, int m, float sum) {
+      const int j = j0 + 16 * tile + n;
+      if (m < count && j < a.rank) s[static_cast<int64_t>(rowS[m]) * a.rank + j] = sum;
+    });
+    __syncthreads();  // before the next block's tiles
+  }
 }
 
 template <class T, bool EVEN, int NT>
 __global__ __launch_bounds__(kThreads) void adapter_down_kernel(const Adapters<T> a) {
   __shared__ Meet<NT> meet;
   __shared__ int rowS[16];
-  down_body<T, EVEN, NT>(a, blockIdx.x, blockIdx.y, blockIdx.z, meet, rowS);
+  down_body<T, EVEN, NT>(a, blockIdx.x, blockIdx.y, blockIdx.z, gridDim.z, meet, rowS);
 }
 
 // x W^T of 16 NT weight rows and 16 MT rows of x over a part of the columns, in f32.
@@ -535,7 +542,7 @@ __global__ __launch_bounds__(kThreads) void adapter_both_kernel(const Adapters<T
     wide_body<T, MT, NT>(a, b, lds.wide);
   } else {
     const int d = b - wide_blocks, part = d % a.splits, ranks = d / a.splits % rank_blocks;
-    down_body<T, EVEN, NT>(a, d / a.splits / rank_blocks, part, ranks, lds.down.meet, lds.down.rows);
+    down_body<T, EVEN, NT>(a, d / a.splits / rank_blocks, part, ranks, rank_blocks, lds.down.meet, lds.down.rows);
   }
 }
 
@@ -654,16 +661,28 @@ static void launch_up(const Adapters<T>& a, hipStream_t s) {
 template <class T, bool EVEN>
 static void launch_delta(const Adapters<T>& a, bool any_order, hipStream_t s) {
   if (!any_order) {
-    const dim3 grid(static_cast<unsigned>((a.rows + 31) / 32), kRunTurns);
-    if (a.rank <= 16)
-      hipLaunchKernelGGL((adapter_run_kernel<T, EVEN, 1>), grid, dim3(kThreads), 0, s, a);
-    else if (a.rank <= 32)
-      hipLaunchKernelGGL((adapter_run_kernel<T, EVEN, 2>), grid, dim3(kThreads), 0, s, a);
-    else
-      hipLaunchKernelGGL((adapter_run_kernel<T, EVEN, 4>), grid, dim3(kThreads), 0, s, a);
+    // 16 rows a workgroup while 32 would leave CUs empty (2048 -> 2048 rank 16, beside
+    // the projection: 300 rows 9.9 us against 13.8, 2000 15 against 18, 4096 17
+    // against 18, 8195 12 against 9)
+    auto go = [&](auto kernel, int rows) {
+      const dim3 grid(static_cast<unsigned>((a.rows + rows - 1) / rows), kRunTurns);
+      hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, a);
+    };
+    if (a.rows <= 4096) {
+      if (a.rank <= 16) go(adapter_run_kernel<T, EVEN, 1, 1>, 16);
+      else if (a.rank <= 32) go(adapter_run_kernel<T, EVEN, 1, 2>, 16);
+      else go(adapter_run_kernel<T, EVEN, 1, 4>, 16);
+    } else {
+      if (a.rank <= 16) go(adapter_run_kernel<T, EVEN, 2, 1>, 32);
+      else if (a.rank <= 32) go(adapter_run_kernel<T, EVEN, 2, 2>, 32);
+      else go(adapter_run_kernel<T, EVEN, 2, 4>, 32);
+    }
     return;
   }
-  const dim3 grid(static_cast<unsigned>(a.rows), a.splits, static_cast<unsigned>((a.rank + 31) / 32));
+  // 32 of the rank a workgroup while all of them run at once: most of many rows'
+  // workgroups have nothing to do, and a second round of them waits
+  const int64_t ranks = (a.rank + 31) / 32, fill = 1024 / (a.rows * a.splits);
+  const dim3 grid(static_cast<unsigned>(a.rows), a.splits, static_cast<unsigned>(fill < 1 ? 1 : fill < ranks ? fill : ranks));
   if (a.rank <= 16)
     hipLaunchKernelGGL((adapter_down_kernel<T, EVEN, 1>), grid, dim3(kThreads), 0, s, a);
   else
