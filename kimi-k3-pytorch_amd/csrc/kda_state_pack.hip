@@ -245,6 +245,8 @@ namespace kda_host {
 
 using namespace kda;
 
+static_assert(sizeof(kda_state_tensor) == 48, "callers may pass records as six words");
+
 static bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
   const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
   return pa < pb + static_cast<uintptr_t>(nb) && pb < pa + static_cast<uintptr_t>(na);

@@ -63,14 +63,7 @@ class AdapterArgs(ctypes.Structure):
     )
 
 
-class StateTensor(ctypes.Structure):
-    """kda_state_tensor, field for field."""
-
-    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("scales", ctypes.c_void_p),
-                ("rows", ctypes.c_int64), ("width", ctypes.c_int64), ("kind", ctypes.c_int)]
-
-
-# kda_state_tensor.kind
+# kda_state_tensor.kind (a record is six words: src, dst, scales, rows, width, kind)
 MOVE_BYTES, MOVE_PACK, MOVE_UNPACK = 0, 1, 2
 
 

@@ -186,18 +186,32 @@ def clone_states(states: Sequence[KDAState]) -> list[KDAState]:
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
-def _move(tensors: list[_lib.StateTensor], dtype: torch.dtype, device: torch.device, src_index, n_src, dst_index, n_dst,
-          n, report=True) -> torch.Tensor | None:
-    """``kda_state_move`` and the status it sets for a slot out of range (None
-    without slots, or into a graph, where no one can read it)."""
-    checked = (report and (src_index is not None or dst_index is not None)
-               and not torch.cuda.is_current_stream_capturing())
-    status = torch.zeros(1, dtype=torch.int32, device=device) if checked else None
+def _moves(tensors: list[tuple[int, int, int | None, int, int, int]]) -> ctypes.Array:
+    """``kda_state_tensor`` records (src, dst, scales, rows, width, kind) as one array of words."""
+    words = []
+    for src, dst, scales, rows, width, kind in tensors:
+        words += (src, dst, scales or 0, rows, width, kind)
+    return (ctypes.c_int64 * len(words))(*words)
+
+
+def _status(device: torch.device, index: torch.Tensor | None) -> torch.Tensor | None:
+    """What the kernels set for a slot out of range: None without slots, or into a
+    graph, where no one can read it."""
+    if index is None or torch.cuda.is_current_stream_capturing():
+        return None
+    return torch.zeros(1, dtype=torch.int32, device=device)
+
+
+def _move(tensors, code: int, src_index, n_src: int, dst_index, n_dst: int, n: int, status, stream: int) -> None:
     if n and tensors:
-        _lib.check(_lib.load().kda_state_move((_lib.StateTensor * len(tensors))(*tensors), len(tensors),
-                                              _lib.dtype_code(dtype), _lib.ptr(src_index), n_src, _lib.ptr(dst_index),
-                                              n_dst, n, _lib.ptr(status), _prep.stream(device)))
-    return status
+        _lib.check(_lib.load().kda_state_move(_moves(tensors), len(tensors), code, _lib.ptr(src_index), n_src,
+                                              _lib.ptr(dst_index), n_dst, n, _lib.ptr(status), stream))
+
+
+# Bytes of f32 states that a launch waits for, so that the GPU starts while the host
+# makes the records and outputs of the layers behind (8 layers of 64 MiB: 286 us a
+# store with launches of two layers, 296 us in one, 307 us with one for each).
+LAUNCH_BYTES = 100 << 20
 
 
 def _check_slots(status: torch.Tensor | None, slots: int) -> None:
@@ -215,16 +229,17 @@ def _slots_arg(slots: torch.Tensor | None, device: torch.device) -> torch.Tensor
     return slots.contiguous()
 
 
-def _bytes(src: torch.Tensor, dst: torch.Tensor) -> _lib.StateTensor:
+def _bytes(src: torch.Tensor, dst: torch.Tensor) -> tuple:
     entries = src.shape[0]
-    width = src.numel() // entries * src.element_size() if entries else 0
-    return _lib.StateTensor(src.data_ptr(), dst.data_ptr(), None, 1, width, _lib.MOVE_BYTES)
+    return (src.data_ptr(), dst.data_ptr(), 0, 1, src.nbytes // entries if entries else 0,
+            _lib.MOVE_BYTES)
 
 
 def _one_device(tensors: Sequence[torch.Tensor]) -> torch.device:
     device = tensors[0].device
+    if device.type != "cuda":
+        _lib.require_gpu(tensors[0])
     for t in tensors:
-        _lib.require_gpu(t)
         if t.device != device:
             raise ValueError("all cache tensors must be on one device")
     return device
@@ -236,12 +251,15 @@ def pack_recurrent(state: torch.Tensor) -> PackedState:
     and holds the nearest whole multiples of it (halves to even).  A row whose
     largest magnitude is under 2^-100 reads back as zeros, one with a value
     that is not finite as NaN.  No gradient: raises for a state that needs one."""
-    _check_packable([state])
+    _check_packable(state)
+    if torch.is_grad_enabled() and state.requires_grad:
+        raise RuntimeError("packing has no backward; pack a detached state or call it under torch.no_grad()")
     _one_device([state])
     out = _empty_packed(state, state.shape[0])
+    n = state.shape[0]
     with _prep.on_device(state.device):
         st = state.contiguous()
-        _move([_pack(st, out)], st.dtype, st.device, None, st.shape[0], None, st.shape[0], st.shape[0])
+        _move([_pack(st, out)], _lib.dtype_code(st.dtype), None, n, None, n, n, None, _prep.stream(st.device))
     return out
 
 
@@ -258,7 +276,9 @@ def unpack_recurrent(packed: PackedState, slots: torch.Tensor | None = None,
     _check_entries(n, entries)
     out = torch.empty(n, *rest, dtype=dtype, device=device)
     with _prep.on_device(device):
-        _check_slots(_move([_unpack(packed, out)], dtype, device, slots, entries, None, n, n), entries)
+        status = _status(device, slots)
+        _move([_unpack(packed, out)], _lib.dtype_code(dtype), slots, entries, None, n, n, status, _prep.stream(device))
+        _check_slots(status, entries)
     return out
 
 
@@ -269,7 +289,8 @@ def read_slots(packed: PackedState, slots: torch.Tensor | None) -> torch.Tensor:
     n = entries if slots is None else slots.shape[0]
     out = torch.empty(n, *packed.values.shape[1:], dtype=torch.float32, device=_one_device([packed.values]))
     with _prep.on_device(out.device):
-        _move([_unpack(packed, out)], torch.float32, out.device, slots, entries, None, n, n, report=False)
+        _move([_unpack(packed, out)], _lib.dtype_code(torch.float32), slots, entries, None, n, n, None,
+              _prep.stream(out.device))
     return out
 
 
@@ -306,16 +327,24 @@ def pack_states(states: Sequence[KDAState], *, out: Sequence[PackedKDAState] | N
         raise ValueError(f"the pool has {len(out)} layers, the caches {len(states)}")
     if not states:
         return []
-    flat = [t for s in states for t in _flatten(s)]
-    _check_packable([s.recurrent_state for s in states])
-    if torch.is_grad_enabled() and any(t.requires_grad for t in flat):
-        raise RuntimeError("pack_states has no backward; call it on detached states or under torch.no_grad()")
-    device = _one_device(flat)
-    batch, dtype = flat[0].shape[0], flat[0].dtype
-    if any(t.shape[0] != batch for t in flat):
-        raise ValueError("all cache tensors must share the batch size")
-    if any(s.recurrent_state.dtype != dtype for s in states):
-        raise TypeError("the recurrent states of all layers must share one dtype")
+    layers = [_flatten(s) for s in states]
+    shapes = [t.shape for t in layers[0]]
+    dtypes = [t.dtype for t in layers[0]]
+    _check_packable(layers[0][0])
+    device, batch = layers[0][0].device, shapes[0][0]
+    if device.type != "cuda":
+        _lib.require_gpu(layers[0][0])
+    grad = torch.is_grad_enabled()
+    for layer in layers:
+        if layer[0].dtype != dtypes[0]:
+            raise TypeError("the recurrent states of all layers must share one dtype")
+        for t in layer:
+            if t.device != device:
+                raise ValueError("all cache tensors must be on one device")
+            if t.shape[0] != batch:
+                raise ValueError("all cache tensors must share the batch size")
+            if grad and t.requires_grad:
+                raise RuntimeError("pack_states has no backward; call it on detached states or under torch.no_grad()")
     slots = _slots_arg(slots, device)
     if slots is not None and slots.shape[0] != batch:
         raise ValueError(f"slots must name a slot for each of {batch} batch rows, got {slots.shape[0]}")
@@ -327,30 +356,38 @@ def pack_states(states: Sequence[KDAState], *, out: Sequence[PackedKDAState] | N
                                       conv(s.k_conv_state), conv(s.v_conv_state),
                                       torch.empty_like(s.sequence_offset, memory_format=torch.contiguous_format)))
     out = list(out)
-    entries = out[0].recurrent.values.shape[0]
+    pools = [_packed_parts(p) for p in out]
+    pool_shapes = [t.shape for t in pools[0]]
+    entries = pool_shapes[0][0]
     if slots is None and entries != batch:
         raise ValueError(f"a batch of {batch} needs slots for a pool of {entries}")
     _check_entries(batch, entries)
-    moves, keep = [], []
-    for s, p in zip(states, out):
-        src = [_rows(t) for t in _flatten(s)]
-        dst = _packed_parts(p)
-        keep.append(src)
-        if p.recurrent.values.shape != (entries, *src[0].shape[1:]):
-            raise ValueError(f"pool values must have shape {(entries, *src[0].shape[1:])}, "
-                             f"got {tuple(p.recurrent.values.shape)}")
-        for a, b in zip(src[1:], dst[1:]):
-            if b.shape != (entries, *a.shape[1:]) or b.dtype != a.dtype:
-                raise ValueError(f"pool tensors must have shape {(entries, *a.shape[1:])} and dtype {a.dtype}, "
-                                 f"got {tuple(b.shape)} and {b.dtype}")
+    for i, (src, dst) in enumerate(zip(layers, pools)):  # every layer, before any is written
+        for k, (a, b) in enumerate(zip(src, dst)):
+            if i == 0 or a.shape != shapes[k] or b.shape != pool_shapes[k] or a.dtype != dtypes[k]:
+                expected = torch.int8 if k == 0 else a.dtype
+                if b.shape != (entries, *a.shape[1:]) or b.dtype != expected:
+                    raise ValueError(f"pool tensors must have shape {(entries, *a.shape[1:])} and dtype {expected}, "
+                                     f"got {tuple(b.shape)} and {b.dtype}")
+            elif b.dtype != pools[0][k].dtype:
+                raise ValueError(f"pool tensors must have dtype {pools[0][k].dtype}, got {b.dtype}")
+            if b.device != device:
+                raise ValueError("pool and states must be on the same device")
             if not b.is_contiguous():
                 raise ValueError("pool tensors must be contiguous")
-        if any(b.device != device for b in dst):
-            raise ValueError("pool and states must be on the same device")
-        moves.append(_pack(src[0], p.recurrent))
-        moves += [_bytes(a, b) for a, b in zip(src[1:], dst[1:])]
     with _prep.on_device(device):
-        _check_slots(_move(moves, dtype, device, None, batch, slots, entries, batch), entries)
+        code, stream, status = _lib.dtype_code(dtypes[0]), _prep.stream(device), _status(device, slots)
+        moves, keep, size = [], [], 0
+        for i, (src, dst) in enumerate(zip(layers, pools)):
+            src = [_rows(t) for t in src]
+            keep.append(src)
+            moves.append(_pack(src[0], out[i].recurrent))
+            moves += [_bytes(a, b) for a, b in zip(src[1:], dst[1:])]
+            size += src[0].numel() * 4
+            if size >= LAUNCH_BYTES or i + 1 == len(layers):
+                _move(moves, code, None, batch, slots, entries, batch, status, stream)
+                moves, size = [], 0
+        _check_slots(status, entries)
     return out
 
 
@@ -373,18 +410,23 @@ def unpack_states(packed: Sequence[PackedKDAState], slots: torch.Tensor | None =
         raise ValueError("all layers of a pool must share the number of slots")
     n = entries if slots is None else slots.shape[0]
     _check_entries(n, entries)
-    moves, outs, keep = [], [], []
-    for p, part in zip(packed, parts):
-        rest = [_rows(t) for t in part[1:]]
-        keep.append(rest)
-        new = [torch.empty(n, *p.recurrent.values.shape[1:], dtype=dtype, device=device)]
-        new += [t.new_empty(n, *t.shape[1:]) for t in rest]
-        moves.append(_unpack(p.recurrent, new[0]))
-        moves += [_bytes(a, b) for a, b in zip(rest, new[1:])]
-        outs.append(new)
     with _prep.on_device(device):
-        status = _move(moves, dtype, device, slots, entries, None, n, n)
-        states = [_rebuild(new) for new in outs]  # while the GPU copies
+        code, stream, status = _lib.dtype_code(dtype), _prep.stream(device), _status(device, slots)
+        moves, keep, size, states = [], [], 0, []
+        waiting: list[list[torch.Tensor]] = []  # outputs whose objects are made while the GPU copies
+        for i, (p, part) in enumerate(zip(packed, parts)):
+            rest = [_rows(t) for t in part[1:]]
+            keep.append(rest)
+            new = [torch.empty(n, *part[0].shape[1:], dtype=dtype, device=device)]
+            new += [t.new_empty(n, *t.shape[1:]) for t in rest]
+            moves.append(_unpack(p.recurrent, new[0]))
+            moves += [_bytes(a, b) for a, b in zip(rest, new[1:])]
+            waiting.append(new)
+            size += new[0].numel() * 4
+            if size >= LAUNCH_BYTES or i + 1 == len(packed):
+                _move(moves, code, slots, entries, None, n, n, status, stream)
+                states += [_rebuild(x) for x in waiting]
+                moves, size, waiting = [], 0, []
         _check_slots(status, entries)
     return states
 
@@ -394,14 +436,11 @@ def _check_float(dtype: torch.dtype) -> None:
         raise TypeError(f"recurrent states are read as float32, float16 or bfloat16, not {dtype}")
 
 
-def _check_packable(states: list[torch.Tensor]) -> None:
-    for state in states:
-        if state.ndim != 4:
-            raise ValueError(f"recurrent states must have shape [B,H,K,V], got {tuple(state.shape)}")
-        if state.dtype not in _FLOATS:
-            raise TypeError(f"recurrent states of float32, float16 or bfloat16 are packed, not {state.dtype}")
-        if torch.is_grad_enabled() and state.requires_grad:
-            raise RuntimeError("packing has no backward; pack a detached state or call it under torch.no_grad()")
+def _check_packable(state: torch.Tensor) -> None:
+    if state.ndim != 4:
+        raise ValueError(f"recurrent states must have shape [B,H,K,V], got {tuple(state.shape)}")
+    if state.dtype not in _FLOATS:
+        raise TypeError(f"recurrent states of float32, float16 or bfloat16 are packed, not {state.dtype}")
 
 
 def _check_entries(n: int, entries: int) -> None:
@@ -415,16 +454,16 @@ def _empty_packed(state: torch.Tensor, entries: int) -> PackedState:
                        torch.empty(shape[:3], dtype=torch.float32, device=state.device))
 
 
-def _pack(src: torch.Tensor, dst: PackedState) -> _lib.StateTensor:
+def _pack(src: torch.Tensor, dst: PackedState) -> tuple:
     _, heads, key_dim, value_dim = dst.values.shape
-    return _lib.StateTensor(src.data_ptr(), dst.values.data_ptr(), dst.scales.data_ptr(), heads * key_dim, value_dim,
-                            _lib.MOVE_PACK)
+    return (src.data_ptr(), dst.values.data_ptr(), dst.scales.data_ptr(), heads * key_dim, value_dim,
+            _lib.MOVE_PACK)
 
 
-def _unpack(src: PackedState, dst: torch.Tensor) -> _lib.StateTensor:
+def _unpack(src: PackedState, dst: torch.Tensor) -> tuple:
     _, heads, key_dim, value_dim = src.values.shape
-    return _lib.StateTensor(src.values.data_ptr(), dst.data_ptr(), src.scales.data_ptr(), heads * key_dim, value_dim,
-                            _lib.MOVE_UNPACK)
+    return (src.values.data_ptr(), dst.data_ptr(), src.scales.data_ptr(), heads * key_dim, value_dim,
+            _lib.MOVE_UNPACK)
 
 
 def _packed_parts(p: PackedKDAState) -> list[torch.Tensor]:

@@ -105,13 +105,14 @@ class PackedState:
     scales: torch.Tensor
 
     def __post_init__(self) -> None:
-        if self.values.ndim != 4 or self.values.dtype != torch.int8:
+        values, scales = self.values, self.scales
+        if values.ndim != 4 or values.dtype != torch.int8:
             raise ValueError("packed values must be int8 with shape [N,H,K,V]")
-        if self.scales.shape != self.values.shape[:3] or self.scales.dtype != torch.float32:
-            raise ValueError(f"packed scales must be float32 with shape {tuple(self.values.shape[:3])}")
-        if self.scales.device != self.values.device:
+        if scales.shape != values.shape[:3] or scales.dtype != torch.float32:
+            raise ValueError(f"packed scales must be float32 with shape {tuple(values.shape[:3])}")
+        if scales.device != values.device:
             raise ValueError("packed values and scales must be on the same device")
-        if not (self.values.is_contiguous() and self.scales.is_contiguous()):
+        if not (values.is_contiguous() and scales.is_contiguous()):
             raise ValueError("packed values and scales must be contiguous")
 
 

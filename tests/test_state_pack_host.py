@@ -95,7 +95,7 @@ def test_move_entry_point_rejects_bad_arguments():
 
     def move(src=a, dst=b, scales=c, rows=4, width=8, kind=_lib.MOVE_PACK, dtype=0, n_src=3, n_dst=3, n=3, count=1,
              index=None):
-        t = (_lib.StateTensor * 1)(_lib.StateTensor(src, dst, scales, rows, width, kind))
+        t = cache._moves([(src or 0, dst or 0, scales, rows, width, kind)])
         return lib.kda_state_move(ctypes.addressof(t) if count else None, count, dtype, index, n_src, None, n_dst, n,
                                   None, None)
 
@@ -107,7 +107,7 @@ def test_move_entry_point_rejects_bad_arguments():
         assert move(**kw) == bad, kw
     assert move(n=0) == _lib.KDA_OK and move(count=0) == _lib.KDA_OK
     # two tensors that write one place
-    t = (_lib.StateTensor * 2)(_lib.StateTensor(a, b, None, 1, 8, 0), _lib.StateTensor(c, b + 8, None, 1, 8, 0))
+    t = cache._moves([(a, b, None, 1, 8, 0), (c, b + 8, None, 1, 8, 0)])
     assert lib.kda_state_move(ctypes.addressof(t), 2, 0, None, 3, None, 3, 3, None, None) == bad
 
     def step(values=a, scales=a, slots=None, n_slots=3, dtype=2, q=a):
