@@ -626,6 +626,27 @@ size_t kda_adapter_linear_workspace_bytes(const kda_adapter_args* args);
 
 int kda_adapter_linear(const kda_adapter_args* args, void* stream);
 
+/*
+ * kda_layer_decode with low-rank adapters beside the q, k, v, gate and output projections (in
+ * this order; a[j] NULL: none), for up to 32 sequences: each projection that has a stack runs
+ * as kda_adapter_linear does, with the layer's weight and bias.
+ *   a[j], b[j]  : [adapters[j], rank[j], d_model], [adapters[j], its rows, rank[j]], 16-byte aligned
+ *   scaling[j]  : f32 [adapters[j]] or NULL (1)
+ *   ids         : int32 or int64 [batch], one id for all five
+ * The workspace in `args` is of kda_layer_decode_adapters_workspace_bytes.
+ */
+typedef struct {
+  const void *a[5], *b[5];
+  const float* scaling[5];
+  int64_t rank[5], adapters[5];
+  const void* ids;
+  int64_t ids_are_int64;
+} kda_layer_adapters;
+
+size_t kda_layer_decode_adapters_workspace_bytes(const kda_layer_decode_args* args, const kda_layer_adapters* adapters);
+
+int kda_layer_decode_adapters(const kda_layer_decode_args* args, const kda_layer_adapters* adapters, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -604,13 +604,15 @@ int kda_mask_lengths(const uint8_t* mask, int64_t batch, int64_t tokens, int32_t
   return launch_mask_lengths(mask, batch, tokens, lengths, static_cast<hipStream_t>(stream));
 }
 
-size_t kda_layer_decode_workspace_bytes(const kda_layer_decode_args* args) {
-  if (!args || args->batch <= 0 || args->heads <= 0 || args->key_dim <= 0 || args->value_dim <= 0 || args->rank <= 0)
-    return 0;
-  return layer_decode_workspace_bytes(*args);
+static bool layer_sizes(const kda_layer_decode_args* args) {
+  return args && args->batch > 0 && args->heads > 0 && args->key_dim > 0 && args->value_dim > 0 && args->rank > 0;
 }
 
-int kda_layer_decode(const kda_layer_decode_args* args, void* stream) {
+size_t kda_layer_decode_workspace_bytes(const kda_layer_decode_args* args) {
+  return layer_sizes(args) ? layer_decode_workspace_bytes(*args, nullptr) : 0;
+}
+
+static int check_layer_decode(const kda_layer_decode_args* args) {
   g_detail[0] = '\0';
   if (!args || args->batch <= 0 || args->d_model <= 0 || args->out_dim <= 0 || args->heads <= 0 ||
       args->key_dim <= 0 || args->value_dim <= 0 || args->rank <= 0 || args->taps <= 0) {
@@ -632,7 +634,12 @@ int kda_layer_decode(const kda_layer_decode_args* args, void* stream) {
       set_detail("layer_decode: x, the linear weights, the states and the workspace must be 16-byte aligned");
       return KDA_ERR_INVALID_ARGUMENT;
     }
-  return launch_layer_decode(d, static_cast<hipStream_t>(stream));
+  return KDA_OK;
+}
+
+int kda_layer_decode(const kda_layer_decode_args* args, void* stream) {
+  const int rc = check_layer_decode(args);
+  return rc != KDA_OK ? rc : launch_layer_decode(*args, nullptr, static_cast<hipStream_t>(stream));
 }
 
 static int check_norm(const char* what, const void* in, int64_t rows, int64_t width, double eps, int dtype,
@@ -798,6 +805,36 @@ int kda_adapter_linear(const kda_adapter_args* args, void* stream) {
   }
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return d.weight ? launch_adapter_linear(d, s) : launch_adapter_delta(d, s);
+}
+
+static bool layer_adapter_sizes(const kda_layer_adapters* ad) {
+  if (!ad) return false;
+  for (int j = 0; j < 5; ++j)
+    if (ad->a[j] && (ad->rank[j] < 1 || ad->rank[j] > 256 || ad->adapters[j] < 1 || ad->adapters[j] > 0xffffff))
+      return false;
+  return true;
+}
+
+size_t kda_layer_decode_adapters_workspace_bytes(const kda_layer_decode_args* args,
+                                                 const kda_layer_adapters* adapters) {
+  if (!layer_sizes(args) || args->d_model <= 0 || args->out_dim <= 0 || !layer_adapter_sizes(adapters)) return 0;
+  return layer_decode_workspace_bytes(*args, adapters);
+}
+
+int kda_layer_decode_adapters(const kda_layer_decode_args* args, const kda_layer_adapters* adapters, void* stream) {
+  const int rc = check_layer_decode(args);
+  if (rc != KDA_OK) return rc;
+  if (!layer_adapter_sizes(adapters) || !adapters->ids) {
+    set_detail("layer_decode_adapters: adapters of rank 1..256 (below 2^24 of them) and ids must be given");
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  for (int j = 0; j < 5; ++j)
+    if (adapters->a[j] && (!adapters->b[j] || reinterpret_cast<uintptr_t>(adapters->a[j]) % 16 != 0 ||
+                           reinterpret_cast<uintptr_t>(adapters->b[j]) % 16 != 0)) {
+      set_detail("layer_decode_adapters: a and b must be non-null and 16-byte aligned");
+      return KDA_ERR_INVALID_ARGUMENT;
+    }
+  return launch_layer_decode(*args, adapters, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

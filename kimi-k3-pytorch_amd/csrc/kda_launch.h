@@ -160,9 +160,10 @@ int launch_cache_gather(const void* const* src, void* const* dst, const int64_t*
 int launch_mask_lengths(const uint8_t* mask, int64_t batch, int64_t tokens, int32_t* lengths, hipStream_t stream);
 
 // One decode step of a layer (csrc/kda_layer_decode.hip).
-size_t layer_decode_workspace_bytes(const kda_layer_decode_args& d);
+// `ad`: the projections' adapters, or null.
+size_t layer_decode_workspace_bytes(const kda_layer_decode_args& d, const kda_layer_adapters* ad);
 
-int launch_layer_decode(const kda_layer_decode_args& d, hipStream_t stream);
+int launch_layer_decode(const kda_layer_decode_args& d, const kda_layer_adapters* ad, hipStream_t stream);
 
 // RMSNorm with the residual's addition, plain or e4m3 output (q non-null), and its backward (csrc/kda_norm.hip).
 int launch_add_norm(const void* x, const void* r, const void* w, void* h, void* y, void* q, float* scales,

@@ -1,7 +1,8 @@
 // One decode step of a whole KDA layer in three launches: every projection of
 // the token (multi_linear_kernel), everything between the projections and the
 // output projection per (sequence, head) (layer_core_kernel), and the output
-// projection (multi_linear_kernel again).
+// projection (multi_linear_kernel again).  A projection with low-rank adapters
+// leaves the first or last of them and runs on its own (kda_adapter.hip).
 //
 // Reference: KimiDeltaAttention.forward in decode (src/kda/kda.py:98-183) over
 // KDAProjections.forward (src/kda/projections.py:144-225).  The composition of
@@ -375,10 +376,38 @@ static int64_t decode_elems(const kda_layer_decode_args& d) {
   return d.batch * (2 * kw + 3 * vw + d.heads + d.rank) + 7 * 8;
 }
 
-size_t layer_decode_workspace_bytes(const kda_layer_decode_args& d) { return static_cast<size_t>(decode_elems(d)) * 2; }
+// One projection with its adapters: j of q, k, v, gate, output.
+static kda_adapter_args adapter_call(const kda_layer_decode_args& d, const kda_layer_adapters& ad, int j, const void* x,
+                                     void* y, void* workspace) {
+  const void* weight[5] = {d.q_proj, d.k_proj, d.v_proj, d.gate_proj, d.output_proj};
+  const void* bias[5] = {d.q_bias, d.k_bias, d.v_bias, d.gate_bias, d.output_bias};
+  const int64_t kw = d.heads * d.key_dim, vw = d.heads * d.value_dim, out[5] = {kw, kw, vw, vw, d.out_dim};
+  kda_adapter_args c{};
+  c.x = x, c.weight = weight[j], c.a = ad.a[j], c.b = ad.b[j], c.bias = bias[j], c.scaling = ad.scaling[j];
+  c.ids = ad.ids, c.ids_are_int64 = ad.ids_are_int64 != 0, c.y = y, c.workspace = workspace;
+  c.rows = d.batch, c.span = 1, c.d_in = j < 4 ? d.d_model : vw, c.d_out = out[j];
+  c.rank = ad.rank[j], c.adapters = ad.adapters[j], c.dtype = d.dtype;
+  return c;
+}
+
+static size_t own_bytes(const kda_layer_decode_args& d) {
+  return (static_cast<size_t>(decode_elems(d)) * 2 + 31) / 32 * 32;
+}
+
+size_t layer_decode_workspace_bytes(const kda_layer_decode_args& d, const kda_layer_adapters* ad) {
+  if (ad == nullptr) return static_cast<size_t>(decode_elems(d)) * 2;
+  size_t most = 0;  // the projections take the same piece in turn
+  for (int j = 0; j < 5; ++j)
+    if (ad->a[j] != nullptr) {
+      const size_t n = adapter_workspace_bytes(adapter_call(d, *ad, j, d.x, nullptr, nullptr));
+      most = n > most ? n : most;
+    }
+  return own_bytes(d) + most;
+}
 
 template <class IT>
-static int run_layer_decode(const kda_layer_decode_args& d, hipStream_t s) {
+static int run_layer_decode(const kda_layer_decode_args& d, const kda_layer_adapters* ad, hipStream_t s) {
+  void* const beside = static_cast<char*>(d.workspace) + own_bytes(d);
   const int64_t B = d.batch, H = d.heads, kw = H * d.key_dim, vw = H * d.value_dim;
   IT* p = static_cast<IT*>(d.workspace);
   auto take = [&](int64_t n) {  // 16-byte aligned pieces
@@ -397,10 +426,15 @@ static int run_layer_decode(const kda_layer_decode_args& d, hipStream_t s) {
   const void* bias[kMaxLinear] = {d.beta_bias, nullptr, d.q_bias, d.k_bias, d.v_bias, d.gate_bias};
   IT* y[kMaxLinear] = {bl, dl, ql, kl, vl, gl};
   const int64_t n[kMaxLinear] = {H, d.rank, kw, kw, vw, vw};
-  a.count = kMaxLinear;
-  for (int j = 0; j < kMaxLinear; ++j) {
-    a.w[j] = in(w[j]), a.bias[j] = in(bias[j]), a.y[j] = y[j], a.n[j] = static_cast<int>(n[j]);
-    a.first[j + 1] = a.first[j] + static_cast<int>((n[j] + 31) / 32);
+  for (int t = 0; t < kMaxLinear; ++t) {
+    if (ad != nullptr && t >= 2 && ad->a[t - 2] != nullptr) {
+      const int rc = launch_adapter_linear(adapter_call(d, *ad, t - 2, d.x, y[t], beside), s);
+      if (rc != KDA_OK) return rc;
+      continue;
+    }
+    const int j = a.count++;
+    a.w[j] = in(w[t]), a.bias[j] = in(bias[t]), a.y[j] = y[t], a.n[j] = static_cast<int>(n[t]);
+    a.first[j + 1] = a.first[j] + static_cast<int>((n[t] + 31) / 32);
   }
   launch_linear<IT, 2>(a, s);
   LayerCore<IT> c{};
@@ -424,6 +458,10 @@ static int run_layer_decode(const kda_layer_decode_args& d, hipStream_t s) {
     launch_core<IT, 64, 128>(c, B, s);
   else
     launch_core<IT, 64, 64>(c, B, s);
+  if (ad != nullptr && ad->a[4] != nullptr) {
+    const int rc = launch_adapter_linear(adapter_call(d, *ad, 4, gated, d.out, beside), s);
+    return rc != KDA_OK ? rc : check_launch("layer_decode");
+  }
   MultiLinear<IT> o{};
   o.x = gated, o.M = static_cast<int>(B), o.K = static_cast<int>(vw), o.count = 1;
   o.w[0] = in(d.output_proj), o.bias[0] = in(d.output_bias), o.y[0] = static_cast<IT*>(d.out);
@@ -434,7 +472,7 @@ static int run_layer_decode(const kda_layer_decode_args& d, hipStream_t s) {
   return check_launch("layer_decode");
 }
 
-int launch_layer_decode(const kda_layer_decode_args& d, hipStream_t stream) {
+int launch_layer_decode(const kda_layer_decode_args& d, const kda_layer_adapters* ad, hipStream_t stream) {
   if (d.dtype != KDA_DTYPE_BF16 && d.dtype != KDA_DTYPE_F16) {
     set_detail("layer_decode: bf16 or f16 tensors (dtype %d)", d.dtype);
     return KDA_ERR_UNSUPPORTED;
@@ -446,11 +484,16 @@ int launch_layer_decode(const kda_layer_decode_args& d, hipStream_t stream) {
                "up to 8 ShortConv taps");
     return KDA_ERR_UNSUPPORTED;
   }
-  if (d.workspace_bytes < layer_decode_workspace_bytes(d)) {
-    set_detail("layer_decode: workspace of %zu bytes needed", layer_decode_workspace_bytes(d));
+  for (int j = 0; ad != nullptr && j < 5; ++j)
+    if (ad->a[j] != nullptr && !adapter_takes_projection(adapter_call(d, *ad, j, d.x, nullptr, nullptr))) {
+      set_detail("layer_decode: adapters take up to 32 sequences");
+      return KDA_ERR_UNSUPPORTED;
+    }
+  if (d.workspace_bytes < layer_decode_workspace_bytes(d, ad)) {
+    set_detail("layer_decode: workspace of %zu bytes needed", layer_decode_workspace_bytes(d, ad));
     return KDA_ERR_WORKSPACE;
   }
-  return d.dtype == KDA_DTYPE_BF16 ? run_layer_decode<bf16>(d, stream) : run_layer_decode<f16>(d, stream);
+  return d.dtype == KDA_DTYPE_BF16 ? run_layer_decode<bf16>(d, ad, stream) : run_layer_decode<f16>(d, ad, stream);
 }
 
 }  // namespace kda_host

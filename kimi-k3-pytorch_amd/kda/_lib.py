@@ -63,6 +63,14 @@ class AdapterArgs(ctypes.Structure):
     )
 
 
+class LayerAdapters(ctypes.Structure):
+    """kda_layer_adapters, field for field."""
+
+    _fields_ = [("a", ctypes.c_void_p * 5), ("b", ctypes.c_void_p * 5), ("scaling", ctypes.c_void_p * 5),
+                ("rank", ctypes.c_int64 * 5), ("adapters", ctypes.c_int64 * 5), ("ids", ctypes.c_void_p),
+                ("ids_are_int64", ctypes.c_int64)]
+
+
 # kda_state_tensor.kind (a record is six words: src, dst, scales, rows, width, kind)
 MOVE_BYTES, MOVE_PACK, MOVE_UNPACK = 0, 1, 2
 
@@ -130,6 +138,8 @@ SIGNATURES = {
     "kda_layer_decode": (_I, [_P, _P]),
     "kda_state_move": (_I, [_P, _I, _I, _P, _L, _P, _L, _L, _P, _P]),
     "kda_recurrent_fwd_packed": (_I, [_P] * 5 + [_I, _P, _P, _P, _L, _P, _P, _P, _L, _P] + [_L] * 5 + [_P]),
+    "kda_layer_decode_adapters_workspace_bytes": (_S, [_P, _P]),
+    "kda_layer_decode_adapters": (_I, [_P, _P, _P]),
     "kda_adapter_linear_takes_weight": (_I, [_P]),
     "kda_adapter_linear_workspace_bytes": (_S, [_P]),
     "kda_adapter_linear": (_I, [_P, _P]),

@@ -142,4 +142,35 @@ class KDALayerAdapters:
     output_proj: AdapterStack | None = None
 
 
+_LAYER = ("q_proj", "k_proj", "v_proj", "gate_proj", "output_proj")
+STEP_ROWS = 32  # rows whose projections the kernels form themselves
+
+
+def layer_step_args(w, x: torch.Tensor, stacks: KDALayerAdapters, adapter_ids: torch.Tensor):
+    """``kda_layer_adapters`` of a decode step on ``x [B,1,d_model]``, or None where the
+    call needs the single projections (more rows, other layouts); raises what
+    ``adapter_linear`` raises."""
+    rank, count = [0] * 5, [0] * 5
+    a, b, scaling = [None] * 5, [None] * 5, [None] * 5
+    native = x.shape[0] <= STEP_ROWS and adapter_ids.is_contiguous()
+    for j, name in enumerate(_LAYER):
+        stack = getattr(stacks, name)
+        if stack is None:
+            continue
+        _check(x, getattr(w, name), getattr(w, name + "_bias" if j in (0, 1, 2) else name[:-5] + "_bias"), stack,
+               adapter_ids)
+        a[j], b[j] = stack.a.data_ptr(), stack.b.data_ptr()
+        if not (stack.a.is_contiguous() and stack.b.is_contiguous()) or (a[j] | b[j]) & 15:
+            native = False
+        if stack.scaling is not None:
+            scaling[j] = stack.scaling.data_ptr()
+            native = native and stack.scaling.is_contiguous()
+        count[j], rank[j] = stack.a.shape[0], stack.a.shape[1]
+    if not native:
+        return None
+    P, L = ctypes.c_void_p * 5, ctypes.c_int64 * 5
+    return _lib.LayerAdapters(P(*a), P(*b), P(*scaling), L(*rank), L(*count), adapter_ids.data_ptr(),
+                              1 if adapter_ids.dtype == torch.int64 else 0)
+
+
 __all__ = ["AdapterStack", "KDALayerAdapters", "adapter_linear"]

@@ -35,7 +35,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib, _prep, fused
-from .adapters import KDALayerAdapters, adapter_linear
+from .adapters import KDALayerAdapters, adapter_linear, layer_step_args
 from .cache import unpack_states
 from .chunkwise import checked_chunkwise
 from .recurrent import checked_recurrent
@@ -203,8 +203,11 @@ def _transformed() -> bool:
     return torch._C._functorch.peek_interpreter_stack() is not None or torch.autograd.forward_ad._current_level >= 0
 
 
-def _decode_step(w: KDALayerWeights, x: torch.Tensor, state: KDAState | None, in_place: bool) -> KDALayerOutput | None:
-    """One token per sequence through ``kda_layer_decode``, or None when the call
+def _decode_step(w: KDALayerWeights, x: torch.Tensor, state: KDAState | None, in_place: bool,
+                 adapters: KDALayerAdapters | None = None, adapter_ids: torch.Tensor | None = None
+                 ) -> KDALayerOutput | None:
+    """One token per sequence through ``kda_layer_decode`` (with adapters
+    ``kda_layer_decode_adapters``), or None when the call
     needs the composed stages: tensors that require grad, autocast, torch.func
     transforms, tensor subclasses, layouts, dtypes or sizes the kernels do not take, or anything
     the stages would refuse (so that they raise their own errors)."""
@@ -260,6 +263,11 @@ def _decode_step(w: KDALayerWeights, x: torch.Tensor, state: KDAState | None, in
     ptr = [None if t is None else t.data_ptr() for t, _ in expected] + [None] * (29 - len(expected))
     if any(p is not None and p & 15 for p in (*ptr[:9], ptr[27])):
         return None
+    beside = None
+    if adapters is not None:
+        beside = layer_step_args(w, x, adapters, adapter_ids)
+        if beside is None:
+            return None
     lib = _lib.load()
     new = x.new_empty
     outs = [new(*hist, kw), new(*hist, kw), new(*hist, vw)]
@@ -271,10 +279,16 @@ def _decode_step(w: KDALayerWeights, x: torch.Tensor, state: KDAState | None, in
         batch, d_model, out_dim, H, K, V, taps, rank, float(w.g_min), float(w.eps), _lib.dtype_code(dtype),
         1 if per_head else 0)
     ref = ctypes.addressof(args)
-    args.workspace_bytes = lib.kda_layer_decode_workspace_bytes(ref)
+    if beside is None:
+        args.workspace_bytes = lib.kda_layer_decode_workspace_bytes(ref)
+    else:
+        args.workspace_bytes = lib.kda_layer_decode_adapters_workspace_bytes(ref, ctypes.addressof(beside))
     workspace = _prep.workspace(args.workspace_bytes, device, "kda_attention_forward's decode step")
     args.workspace = workspace.data_ptr()
-    _lib.check(lib.kda_layer_decode(ref, _prep.stream(device)))
+    if beside is None:
+        _lib.check(lib.kda_layer_decode(ref, _prep.stream(device)))
+    else:
+        _lib.check(lib.kda_layer_decode_adapters(ref, ctypes.addressof(beside), _prep.stream(device)))
     return KDALayerOutput(hidden_states=out, state=KDAState(
         recurrent_state=state_out, q_conv_state=ShortConvState(outs[0]), k_conv_state=ShortConvState(outs[1]),
         v_conv_state=ShortConvState(outs[2]), sequence_offset=offset_out))
@@ -324,8 +338,8 @@ def kda_attention_forward(
         stack = None if adapters is None else getattr(adapters, name)
         return F.linear(t, weight, bias) if stack is None else adapter_linear(t, weight, bias, stack, adapter_ids)
 
-    if mode == "decode" and attention_mask is None and adapters is None:
-        step = _decode_step(w, x, state, update_state_in_place)
+    if mode == "decode" and attention_mask is None:
+        step = _decode_step(w, x, state, update_state_in_place, adapters, adapter_ids)
         if step is not None:
             return step
     H, K, V = w.num_heads, w.key_head_dim, w.value_head_dim

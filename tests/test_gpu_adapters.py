@@ -240,3 +240,74 @@ def test_a_served_request_end_to_end():
             assert float((kept.recurrent_state - rest.recurrent_state).abs().max()) <= \
                 float(pool[0].recurrent.scales[slots].max()) * K ** 0.5
             assert torch.equal(kept.sequence_offset, rest.sequence_offset)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("batch", [1, 5, 17, 32, 40])
+@pytest.mark.parametrize("which", [("q_proj", "k_proj", "v_proj", "gate_proj", "output_proj"), ("v_proj",),
+                                   ("k_proj", "output_proj"), ()])
+def test_a_decode_step_with_adapters_is_the_composed_stages(batch, dtype, which):
+    # up to 32 sequences run the native step, whose projections are the same kernels
+    # as adapter_linear's; the stages around them round at the same places
+    d_model, H, K = 256, 2, 128
+    weights = layer_weights(d_model, H, K, K, dtype=dtype, biases=True, std=0.06)
+    w = KDALayerWeights(**{n: t.to(DEV) if isinstance(t, torch.Tensor) else t for n, t in weights.items()})
+    gen = torch.Generator().manual_seed(5)
+    rnd = lambda *s, std=1.0: (torch.randn(*s, generator=gen) * std).to(dtype).to(DEV)  # noqa: E731
+    stacks = {n: adapters.AdapterStack(rnd(4, 8 + 4 * i, d_model, std=0.06), rnd(4, d_model, 8 + 4 * i, std=0.1),
+                                       torch.rand(4, generator=gen).to(DEV) if i % 2 else None)
+              for i, n in enumerate(which)}
+    lora = kda.adapters.KDALayerAdapters(**stacks)
+    ids = torch.randint(-1, 4, (batch,), generator=gen).to(DEV)
+    state = kda_attention_forward(w, rnd(batch, 9, d_model), None, None, "chunkwise", True).state
+    x = rnd(batch, 1, d_model)
+    mask = torch.ones(batch, 1, dtype=torch.bool, device=DEV)  # a mask keeps the composed stages
+    want = kda_attention_forward(w, x, mask, state, "decode", adapters=lora, adapter_ids=ids)
+    kept = state.recurrent_state.clone()
+    got = kda_attention_forward(w, x, None, state, "decode", adapters=lora, adapter_ids=ids)
+    assert torch.equal(state.recurrent_state, kept)
+    tol = 4 * torch.finfo(dtype).eps  # a few roundings that may fall to the other side
+    for a, b in ((got.hidden_states, want.hidden_states), (got.state.recurrent_state, want.state.recurrent_state),
+                 (got.state.v_conv_state.buffer, want.state.v_conv_state.buffer)):
+        assert float((a.double() - b.double()).abs().max()) <= tol * float(b.double().abs().max())
+    assert torch.equal(got.state.sequence_offset, want.state.sequence_offset)
+    again = kda_attention_forward(w, x, None, state, "decode", update_state_in_place=True, adapters=lora,
+                                  adapter_ids=ids.int())
+    assert again.state.recurrent_state is state.recurrent_state
+    assert torch.equal(again.hidden_states, got.hidden_states)
+    if which:
+        bad = ids.clone()
+        bad[0] = 99
+        out = kda_attention_forward(w, x, None, want.state, "decode", adapters=lora, adapter_ids=bad).hidden_states
+        assert bool(out[0].isnan().any()) and bool(out[1:].isfinite().all())
+
+
+def test_a_captured_decode_step_with_adapters_replays_with_other_ids():
+    d_model, H, K = 256, 2, 128
+    weights = layer_weights(d_model, H, K, K, dtype=torch.bfloat16, std=0.06)
+    w = KDALayerWeights(**{n: t.to(DEV) if isinstance(t, torch.Tensor) else t for n, t in weights.items()})
+    gen = torch.Generator().manual_seed(6)
+    rnd = lambda *s, std=1.0: (torch.randn(*s, generator=gen) * std).to(torch.bfloat16).to(DEV)  # noqa: E731
+    stack = adapters.AdapterStack(rnd(4, 16, d_model, std=0.06), rnd(4, d_model, 16, std=0.1))
+    lora = kda.adapters.KDALayerAdapters(q_proj=stack, output_proj=stack)
+    ids = torch.tensor([1, 0, 3], device=DEV)
+    state = kda_attention_forward(w, rnd(3, 9, d_model), None, None, "chunkwise", True).state
+    x = rnd(3, 1, d_model)
+    step = lambda: kda_attention_forward(w, x, None, state, "decode", adapters=lora, adapter_ids=ids)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for new in ([2, 2, 2], [-1, 3, 0], [0, -1, -1]):
+        ids.copy_(torch.tensor(new))
+        x.copy_(rnd(3, 1, d_model))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        assert torch.equal(out.hidden_states, want.hidden_states)
+        assert torch.equal(out.state.recurrent_state, want.state.recurrent_state)
