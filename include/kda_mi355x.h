@@ -628,8 +628,8 @@ int kda_adapter_linear(const kda_adapter_args* args, void* stream);
 
 /*
  * kda_layer_decode with low-rank adapters beside the q, k, v, gate and output projections (in
- * this order; a[j] NULL: none), for up to 32 sequences: each projection that has a stack runs
- * as kda_adapter_linear does, with the layer's weight and bias.
+ * this order; a[j] NULL: none), for up to 32 sequences, in five launches: the projections run as
+ * kda_adapter_linear's do, with the layer's weights and biases.
  *   a[j], b[j]  : [adapters[j], rank[j], d_model], [adapters[j], its rows, rank[j]], 16-byte aligned
  *   scaling[j]  : f32 [adapters[j]] or NULL (1)
  *   ids         : int32 or int64 [batch], one id for all five

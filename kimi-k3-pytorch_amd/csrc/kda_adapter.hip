@@ -94,6 +94,7 @@ constexpr int kNone = -1, kMissing = -2, kNoRow = -3;
 // the row's adapter, kNone or kMissing
 template <class T>
 __device__ __forceinline__ int adapter_of(const Adapters<T>& a, int64_t row) {
+  if (a.n == 0) return kNone;
   const unsigned i = static_cast<unsigned>(row) / static_cast<unsigned>(a.span);  // rows < 2^31
   const int64_t id = a.ids64 != 0 ? static_cast<const int64_t*>(a.ids)[i] : static_cast<const int32_t*>(a.ids)[i];
   return id < 0 ? kNone : (id < a.n ? static_cast<int>(id) : kMissing);
@@ -524,11 +525,24 @@ __device__ __forceinline__ void wide_body(const Adapters<T>& a, int block, Meet<
   });
 }
 
+// Several projections of few rows (one, or those of a layer's decode step).
+constexpr int kMaxSet = 6;
+
+template <class T>
+struct AdapterSet {
+  Adapters<T> p[kMaxSet];
+  int first[kMaxSet + 1];  // workgroups of projection j
+  int wide[kMaxSet];       // of them those that form x W^T
+  int ranks[kMaxSet];      // blocks of 32 of the rank
+  bool even[kMaxSet];
+  int count;
+};
+
 // Both in one launch, for up to 16 MT rows: workgroups that form s and workgroups
 // that form x W^T.  Neither waits for the other, and the weights, whose bytes
 // bound the call, are read while s is formed.
-template <class T, bool EVEN, int MT>
-__global__ __launch_bounds__(kThreads) void adapter_both_kernel(const Adapters<T> a, int wide_blocks, int rank_blocks) {
+template <class T, int MT>
+__global__ __launch_bounds__(kThreads) void adapter_both_kernel(const AdapterSet<T> set) {
   constexpr int NT = 2;
   __shared__ union {
     Meet<NT * MT> wide;
@@ -537,21 +551,27 @@ __global__ __launch_bounds__(kThreads) void adapter_both_kernel(const Adapters<T
       int rows[16];
     } down;
   } lds;
-  const int b = static_cast<int>(blockIdx.x);
-  if (b < wide_blocks) {
+  const int block = static_cast<int>(blockIdx.x);
+  int j = 0;
+  while (j + 1 < set.count && block >= set.first[j + 1]) ++j;
+  const Adapters<T>& a = set.p[j];
+  const int b = block - set.first[j];
+  if (b < set.wide[j]) {
     wide_body<T, MT, NT>(a, b, lds.wide);
-  } else {
-    const int d = b - wide_blocks, part = d % a.splits, ranks = d / a.splits % rank_blocks;
-    down_body<T, EVEN, NT>(a, d / a.splits / rank_blocks, part, ranks, rank_blocks, lds.down.meet, lds.down.rows);
+    return;
   }
+  const int d = b - set.wide[j], part = d % a.splits, ranks = d / a.splits % set.ranks[j];
+  const int row = d / a.splits / set.ranks[j];
+  if (set.even[j])
+    down_body<T, true, NT>(a, row, part, ranks, set.ranks[j], lds.down.meet, lds.down.rows);
+  else
+    down_body<T, false, NT>(a, row, part, ranks, set.ranks[j], lds.down.meet, lds.down.rows);
 }
 
 // y of 16 rows with one id (an adapter, none, or a missing one), the workgroup's four
 // waves 64 columns each in turn.
 template <class T, bool EVEN, bool WIDE>
-__global__ __launch_bounds__(256) void adapter_up_kernel(const Adapters<T> a) {
-  __shared__ LowRows<T, 16, kMaxRank> low;
-  __shared__ int rowS[16];
+__device__ __forceinline__ void up_body(const Adapters<T>& a, LowRows<T, 16, kMaxRank>& low, int* rowS) {
   const int id = adapter_of(a, blockIdx.x), count = gather_rows<16>(a, blockIdx.x, id, rowS);
   if (count == 0) return;
   const int c0 = 64 * (4 * blockIdx.y + (threadIdx.x >> 6));
@@ -589,6 +609,25 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const Adapters<T> a) {
   up_all<T, EVEN, WIDE, 1>(a, id, c, first, low, rows, c0, 256 * gridDim.y);
 }
 
+template <class T, bool EVEN>
+__global__ __launch_bounds__(256) void adapter_up_kernel(const Adapters<T> a) {
+  __shared__ LowRows<T, 16, kMaxRank> low;
+  __shared__ int rowS[16];
+  up_body<T, EVEN, false>(a, low, rowS);
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void adapter_up_set_kernel(const AdapterSet<T> set) {
+  __shared__ LowRows<T, 16, kMaxRank> low;
+  __shared__ int rowS[16];
+  const Adapters<T>& a = set.p[blockIdx.z];
+  if (256 * static_cast<int>(blockIdx.y) >= a.out) return;
+  if (set.even[blockIdx.z])
+    up_body<T, true, true>(a, low, rowS);
+  else
+    up_body<T, false, true>(a, low, rowS);
+}
+
 }  // namespace kda
 
 namespace kda_host {
@@ -621,7 +660,7 @@ bool adapter_takes_projection(const kda_adapter_args& d) {
 }
 
 static int64_t s_floats(const kda_adapter_args& d) {
-  return by_adapter(d) ? (static_cast<int64_t>(column_splits(d)) * d.rows * d.rank + 7) / 8 * 8 : 0;
+  return by_adapter(d) && d.adapters > 0 ? (static_cast<int64_t>(column_splits(d)) * d.rows * d.rank + 7) / 8 * 8 : 0;
 }
 
 size_t adapter_workspace_bytes(const kda_adapter_args& d) {
@@ -650,12 +689,9 @@ static bool even_call(const kda_adapter_args& d) {
 }
 
 // Workgroups along the columns: about a thousand in all, whose rows are found once.
-template <class T, bool EVEN, bool WIDE>
-static void launch_up(const Adapters<T>& a, hipStream_t s) {
-  const int64_t blocks = (a.out + 255) / 256, fill = (1023 + a.rows) / a.rows;
-  hipLaunchKernelGGL((adapter_up_kernel<T, EVEN, WIDE>),
-                     dim3(static_cast<unsigned>(a.rows), static_cast<unsigned>(blocks < fill ? blocks : fill)), dim3(256),
-                     0, s, a);
+static unsigned up_blocks(int64_t out, int64_t rows) {
+  const int64_t blocks = (out + 255) / 256, fill = (1023 + rows) / rows;
+  return static_cast<unsigned>(blocks < fill ? blocks : fill);
 }
 
 template <class T, bool EVEN>
@@ -687,18 +723,8 @@ static void launch_delta(const Adapters<T>& a, bool any_order, hipStream_t s) {
     hipLaunchKernelGGL((adapter_down_kernel<T, EVEN, 1>), grid, dim3(kThreads), 0, s, a);
   else
     hipLaunchKernelGGL((adapter_down_kernel<T, EVEN, 2>), grid, dim3(kThreads), 0, s, a);
-  launch_up<T, EVEN, false>(a, s);
-}
-
-template <class T, bool EVEN>
-static void launch_both(const Adapters<T>& a, hipStream_t s) {
-  const int wide = a.parts * ((a.out + 31) / 32), ranks = (a.rank + 31) / 32;  // 2^30 workgroups at most
-  const dim3 grid(static_cast<unsigned>(wide + a.rows * a.splits * ranks));
-  if (a.rows <= 16)
-    hipLaunchKernelGGL((adapter_both_kernel<T, EVEN, 1>), grid, dim3(kThreads), 0, s, a, wide, ranks);
-  else
-    hipLaunchKernelGGL((adapter_both_kernel<T, EVEN, 2>), grid, dim3(kThreads), 0, s, a, wide, ranks);
-  launch_up<T, EVEN, true>(a, s);
+  hipLaunchKernelGGL((adapter_up_kernel<T, EVEN>), dim3(static_cast<unsigned>(a.rows), up_blocks(a.out, a.rows)),
+                     dim3(256), 0, s, a);
 }
 
 template <class T>
@@ -720,18 +746,45 @@ int launch_adapter_delta(const kda_adapter_args& d, hipStream_t s) {
 }
 
 template <class T>
-static int run_adapter_linear(const kda_adapter_args& d, hipStream_t s) {
-  Adapters<T> a = adapters_of<T>(d);
-  a.weight = static_cast<const T*>(d.weight), a.wide = a.s + s_floats(d), a.parts = wide_parts(d);
-  if (even_call(d))
-    launch_both<T, true>(a, s);
+static int run_adapter_set(const kda_adapter_args* calls, int count, hipStream_t s) {
+  AdapterSet<T> set{};
+  set.count = count;
+  int64_t blocks = 0;
+  unsigned columns = 1;
+  for (int j = 0; j < count; ++j) {
+    const kda_adapter_args& d = calls[j];
+    Adapters<T>& a = set.p[j];
+    a = adapters_of<T>(d);
+    a.weight = static_cast<const T*>(d.weight), a.wide = a.s + s_floats(d), a.parts = wide_parts(d);
+    set.even[j] = even_call(d);
+    set.first[j] = static_cast<int>(blocks);
+    set.wide[j] = a.parts * ((a.out + 31) / 32);  // 2^30 at most
+    set.ranks[j] = (a.rank + 31) / 32;
+    blocks += set.wide[j] + (a.n != 0 ? a.rows * a.splits * set.ranks[j] : 0);
+    if (blocks > 0x7fffffffLL) {
+      set_detail("adapter_linear: grid too large");
+      return KDA_ERR_UNSUPPORTED;
+    }
+    const unsigned n = up_blocks(a.out, a.rows * count);
+    columns = n > columns ? n : columns;
+  }
+  set.first[count] = static_cast<int>(blocks);
+  const int64_t rows = calls[0].rows;
+  if (rows <= 16)
+    hipLaunchKernelGGL((adapter_both_kernel<T, 1>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, s, set);
   else
-    launch_both<T, false>(a, s);
+    hipLaunchKernelGGL((adapter_both_kernel<T, 2>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, s, set);
+  hipLaunchKernelGGL((adapter_up_set_kernel<T>), dim3(static_cast<unsigned>(rows), columns, count), dim3(256), 0, s, set);
   return check_launch("adapter_linear");
 }
 
-int launch_adapter_linear(const kda_adapter_args& d, hipStream_t s) {
-  return d.dtype == KDA_DTYPE_BF16 ? run_adapter_linear<bf16>(d, s) : run_adapter_linear<f16>(d, s);
+int launch_adapter_set(const kda_adapter_args* calls, int count, hipStream_t s) {
+  if (count > kMaxSet) {
+    set_detail("adapter_linear: %d projections at once", count);
+    return KDA_ERR_UNSUPPORTED;
+  }
+  return calls[0].dtype == KDA_DTYPE_BF16 ? run_adapter_set<bf16>(calls, count, s)
+                                          : run_adapter_set<f16>(calls, count, s);
 }
 
 }  // namespace kda_host

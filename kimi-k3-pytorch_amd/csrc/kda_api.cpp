@@ -804,7 +804,7 @@ int kda_adapter_linear(const kda_adapter_args* args, void* stream) {
     return KDA_ERR_INVALID_ARGUMENT;
   }
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  return d.weight ? launch_adapter_linear(d, s) : launch_adapter_delta(d, s);
+  return d.weight ? launch_adapter_set(&d, 1, s) : launch_adapter_delta(d, s);
 }
 
 static bool layer_adapter_sizes(const kda_layer_adapters* ad) {

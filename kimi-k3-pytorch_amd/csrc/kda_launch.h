@@ -191,6 +191,8 @@ size_t adapter_workspace_bytes(const kda_adapter_args& d);
 
 int launch_adapter_delta(const kda_adapter_args& d, hipStream_t stream);
 
-int launch_adapter_linear(const kda_adapter_args& d, hipStream_t stream);
+// Projections of the same few rows (adapter_takes_projection of each), up to six, each with
+// adapters or (adapters == 0) without, in two launches.
+int launch_adapter_set(const kda_adapter_args* calls, int count, hipStream_t stream);
 
 }  // namespace kda_host

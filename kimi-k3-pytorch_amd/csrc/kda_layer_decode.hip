@@ -1,8 +1,8 @@
 // One decode step of a whole KDA layer in three launches: every projection of
 // the token (multi_linear_kernel), everything between the projections and the
 // output projection per (sequence, head) (layer_core_kernel), and the output
-// projection (multi_linear_kernel again).  A projection with low-rank adapters
-// leaves the first or last of them and runs on its own (kda_adapter.hip).
+// projection (multi_linear_kernel again).  With low-rank adapters the first and the
+// last are two launches each (kda_adapter.hip).
 //
 // Reference: KimiDeltaAttention.forward in decode (src/kda/kda.py:98-183) over
 // KDAProjections.forward (src/kda/projections.py:144-225).  The composition of
@@ -376,38 +376,36 @@ static int64_t decode_elems(const kda_layer_decode_args& d) {
   return d.batch * (2 * kw + 3 * vw + d.heads + d.rank) + 7 * 8;
 }
 
-// One projection with its adapters: j of q, k, v, gate, output.
-static kda_adapter_args adapter_call(const kda_layer_decode_args& d, const kda_layer_adapters& ad, int j, const void* x,
-                                     void* y, void* workspace) {
-  const void* weight[5] = {d.q_proj, d.k_proj, d.v_proj, d.gate_proj, d.output_proj};
-  const void* bias[5] = {d.q_bias, d.k_bias, d.v_bias, d.gate_bias, d.output_bias};
-  const int64_t kw = d.heads * d.key_dim, vw = d.heads * d.value_dim, out[5] = {kw, kw, vw, vw, d.out_dim};
+// Projection j (q, k, v, gate, output, beta, alpha_down) with its adapters, or none.
+static kda_adapter_args adapter_call(const kda_layer_decode_args& d, const kda_layer_adapters& ad, int j) {
+  const void* weight[7] = {d.q_proj, d.k_proj, d.v_proj, d.gate_proj, d.output_proj, d.beta_proj, d.alpha_down};
+  const void* bias[7] = {d.q_bias, d.k_bias, d.v_bias, d.gate_bias, d.output_bias, d.beta_bias, nullptr};
+  const int64_t kw = d.heads * d.key_dim, vw = d.heads * d.value_dim;
+  const int64_t out[7] = {kw, kw, vw, vw, d.out_dim, d.heads, d.rank};
   kda_adapter_args c{};
-  c.x = x, c.weight = weight[j], c.a = ad.a[j], c.b = ad.b[j], c.bias = bias[j], c.scaling = ad.scaling[j];
-  c.ids = ad.ids, c.ids_are_int64 = ad.ids_are_int64 != 0, c.y = y, c.workspace = workspace;
-  c.rows = d.batch, c.span = 1, c.d_in = j < 4 ? d.d_model : vw, c.d_out = out[j];
-  c.rank = ad.rank[j], c.adapters = ad.adapters[j], c.dtype = d.dtype;
+  c.x = d.x, c.weight = weight[j], c.bias = bias[j], c.rows = d.batch, c.span = 1, c.dtype = d.dtype;
+  c.d_in = j == 4 ? vw : d.d_model, c.d_out = out[j], c.rank = 1;
+  c.ids = ad.ids, c.ids_are_int64 = ad.ids_are_int64 != 0;
+  if (j < 5 && ad.a[j] != nullptr)
+    c.a = ad.a[j], c.b = ad.b[j], c.scaling = ad.scaling[j], c.rank = ad.rank[j], c.adapters = ad.adapters[j];
   return c;
 }
 
-static size_t own_bytes(const kda_layer_decode_args& d) {
-  return (static_cast<size_t>(decode_elems(d)) * 2 + 31) / 32 * 32;
-}
+static size_t round32(size_t n) { return (n + 31) / 32 * 32; }
 
 size_t layer_decode_workspace_bytes(const kda_layer_decode_args& d, const kda_layer_adapters* ad) {
-  if (ad == nullptr) return static_cast<size_t>(decode_elems(d)) * 2;
-  size_t most = 0;  // the projections take the same piece in turn
-  for (int j = 0; j < 5; ++j)
-    if (ad->a[j] != nullptr) {
-      const size_t n = adapter_workspace_bytes(adapter_call(d, *ad, j, d.x, nullptr, nullptr));
-      most = n > most ? n : most;
-    }
-  return own_bytes(d) + most;
+  const size_t own = static_cast<size_t>(decode_elems(d)) * 2;
+  if (ad == nullptr) return own;
+  size_t inputs = 0;  // side by side; the output projection takes the same piece after them
+  for (int j = 0; j < 7; ++j)
+    if (j != 4) inputs += round32(adapter_workspace_bytes(adapter_call(d, *ad, j)));
+  const size_t output = adapter_workspace_bytes(adapter_call(d, *ad, 4));
+  return round32(own) + (inputs > output ? inputs : output);
 }
 
 template <class IT>
 static int run_layer_decode(const kda_layer_decode_args& d, const kda_layer_adapters* ad, hipStream_t s) {
-  void* const beside = static_cast<char*>(d.workspace) + own_bytes(d);
+  char* const beside = static_cast<char*>(d.workspace) + round32(static_cast<size_t>(decode_elems(d)) * 2);
   const int64_t B = d.batch, H = d.heads, kw = H * d.key_dim, vw = H * d.value_dim;
   IT* p = static_cast<IT*>(d.workspace);
   auto take = [&](int64_t n) {  // 16-byte aligned pieces
@@ -418,25 +416,34 @@ static int run_layer_decode(const kda_layer_decode_args& d, const kda_layer_adap
   IT *ql = take(B * kw), *kl = take(B * kw), *vl = take(B * vw), *gl = take(B * vw), *bl = take(B * H),
      *dl = take(B * d.rank), *gated = take(B * vw);
   auto in = [](const void* q) { return static_cast<const IT*>(q); };
-  MultiLinear<IT> a{};
-  a.x = in(d.x);
-  a.M = static_cast<int>(B);
-  a.K = static_cast<int>(d.d_model);
-  const void* w[kMaxLinear] = {d.beta_proj, d.alpha_down, d.q_proj, d.k_proj, d.v_proj, d.gate_proj};
-  const void* bias[kMaxLinear] = {d.beta_bias, nullptr, d.q_bias, d.k_bias, d.v_bias, d.gate_bias};
-  IT* y[kMaxLinear] = {bl, dl, ql, kl, vl, gl};
-  const int64_t n[kMaxLinear] = {H, d.rank, kw, kw, vw, vw};
-  for (int t = 0; t < kMaxLinear; ++t) {
-    if (ad != nullptr && t >= 2 && ad->a[t - 2] != nullptr) {
-      const int rc = launch_adapter_linear(adapter_call(d, *ad, t - 2, d.x, y[t], beside), s);
-      if (rc != KDA_OK) return rc;
-      continue;
+  if (ad != nullptr) {
+    const int order[kMaxLinear] = {0, 1, 2, 3, 5, 6};
+    IT* y[kMaxLinear] = {ql, kl, vl, gl, bl, dl};
+    kda_adapter_args calls[kMaxLinear];
+    char* piece = beside;
+    for (int t = 0; t < kMaxLinear; ++t) {
+      calls[t] = adapter_call(d, *ad, order[t]);
+      calls[t].y = y[t], calls[t].workspace = piece;
+      piece += round32(adapter_workspace_bytes(calls[t]));
     }
-    const int j = a.count++;
-    a.w[j] = in(w[t]), a.bias[j] = in(bias[t]), a.y[j] = y[t], a.n[j] = static_cast<int>(n[t]);
-    a.first[j + 1] = a.first[j] + static_cast<int>((n[t] + 31) / 32);
+    const int rc = launch_adapter_set(calls, kMaxLinear, s);
+    if (rc != KDA_OK) return rc;
+  } else {
+    MultiLinear<IT> a{};
+    a.x = in(d.x);
+    a.M = static_cast<int>(B);
+    a.K = static_cast<int>(d.d_model);
+    const void* w[kMaxLinear] = {d.beta_proj, d.alpha_down, d.q_proj, d.k_proj, d.v_proj, d.gate_proj};
+    const void* bias[kMaxLinear] = {d.beta_bias, nullptr, d.q_bias, d.k_bias, d.v_bias, d.gate_bias};
+    IT* y[kMaxLinear] = {bl, dl, ql, kl, vl, gl};
+    const int64_t n[kMaxLinear] = {H, d.rank, kw, kw, vw, vw};
+    a.count = kMaxLinear;
+    for (int j = 0; j < kMaxLinear; ++j) {
+      a.w[j] = in(w[j]), a.bias[j] = in(bias[j]), a.y[j] = y[j], a.n[j] = static_cast<int>(n[j]);
+      a.first[j + 1] = a.first[j] + static_cast<int>((n[j] + 31) / 32);
+    }
+    launch_linear<IT, 2>(a, s);
   }
-  launch_linear<IT, 2>(a, s);
   LayerCore<IT> c{};
   c.ql = ql, c.kl = kl, c.vl = vl, c.gl = gl, c.bl = bl, c.dl = dl;
   c.alpha_up = in(d.alpha_up);
@@ -459,8 +466,9 @@ static int run_layer_decode(const kda_layer_decode_args& d, const kda_layer_adap
   else
     launch_core<IT, 64, 64>(c, B, s);
   if (ad != nullptr && ad->a[4] != nullptr) {
-    const int rc = launch_adapter_linear(adapter_call(d, *ad, 4, gated, d.out, beside), s);
-    return rc != KDA_OK ? rc : check_launch("layer_decode");
+    kda_adapter_args call = adapter_call(d, *ad, 4);
+    call.x = gated, call.y = d.out, call.workspace = beside;
+    return launch_adapter_set(&call, 1, s);
   }
   MultiLinear<IT> o{};
   o.x = gated, o.M = static_cast<int>(B), o.K = static_cast<int>(vw), o.count = 1;
@@ -484,8 +492,8 @@ int launch_layer_decode(const kda_layer_decode_args& d, const kda_layer_adapters
                "up to 8 ShortConv taps");
     return KDA_ERR_UNSUPPORTED;
   }
-  for (int j = 0; ad != nullptr && j < 5; ++j)
-    if (ad->a[j] != nullptr && !adapter_takes_projection(adapter_call(d, *ad, j, d.x, nullptr, nullptr))) {
+  for (int j = 0; ad != nullptr && j < 7; ++j)
+    if (!adapter_takes_projection(adapter_call(d, *ad, j))) {
       set_detail("layer_decode: adapters take up to 32 sequences");
       return KDA_ERR_UNSUPPORTED;
     }
