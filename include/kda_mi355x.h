@@ -518,9 +518,10 @@ int kda_layer_decode(const kda_layer_decode_args* args, void* stream);
  * RMSNorm with the residual's addition, over rows of `width` elements of dtype (any of the
  * four): h = x + residual rounded to the dtype, y = h / sqrt(mean(h^2) + eps) * weight.
  *   residual : [rows, width] or NULL (h is x; h may then be NULL and is not written)
- *   weight   : [width] or NULL;  h, y : [rows, width]; h may be x or residual itself
+ *   weight   : [width] or NULL, of the dtype, or f32 (weight_is_f32) beside f16 or bf16
+ *   h, y     : [rows, width]; h may be x or residual itself
  */
-int kda_add_rmsnorm_fwd(const void* x, const void* residual, const void* weight, void* h, void* y, int64_t rows,
+int kda_add_rmsnorm_fwd(const void* x, const void* residual, const void* weight, int weight_is_f32, void* h, void* y, int64_t rows,
                         int64_t width, double eps, int dtype, void* stream);
 
 /*
@@ -531,18 +532,18 @@ int kda_add_rmsnorm_fwd(const void* x, const void* residual, const void* weight,
  * holds a NaN has scale NaN.
  *   q : OCP e4m3 bytes [rows, width];  scales : f32 [rows, width / group]
  */
-int kda_add_rmsnorm_quant(const void* x, const void* residual, const void* weight, void* h, void* q, float* scales,
+int kda_add_rmsnorm_quant(const void* x, const void* residual, const void* weight, int weight_is_f32, void* h, void* q, float* scales,
                           int64_t group, int64_t rows, int64_t width, double eps, int dtype, void* stream);
 
 /*
  * Backward of kda_add_rmsnorm_fwd: from h (x without a residual) and the gradients d_y and d_h
  * (or NULL) of its outputs, dx (the gradient of x and of the residual alike) and d_weight
- * [width] in the dtype (or NULL), summed in f32 (f64) in a fixed order.
+ * [width] in the weight's dtype (or NULL), summed in f32 (f64) in a fixed order.
  * Workspace: kda_add_rmsnorm_bwd_workspace_bytes(rows, width, dtype), needed with d_weight.
  */
 size_t kda_add_rmsnorm_bwd_workspace_bytes(int64_t rows, int64_t width, int dtype);
 
-int kda_add_rmsnorm_bwd(const void* h, const void* weight, const void* d_y, const void* d_h, void* dx, void* d_weight,
+int kda_add_rmsnorm_bwd(const void* h, const void* weight, int weight_is_f32, const void* d_y, const void* d_h, void* dx, void* d_weight,
                         int64_t rows, int64_t width, double eps, int dtype, void* workspace, size_t workspace_bytes,
                         void* stream);
 

@@ -697,14 +697,14 @@ static unsigned up_blocks(int64_t out, int64_t rows) {
 template <class T, bool EVEN>
 static void launch_delta(const Adapters<T>& a, bool any_order, hipStream_t s) {
   if (!any_order) {
-    // 16 rows a workgroup while 32 would leave CUs empty (2048 -> 2048 rank 16, beside
-    // the projection: 300 rows 9.9 us against 13.8, 2000 15 against 18, 4096 17
-    // against 18, 8195 12 against 9)
+    // 16 rows a workgroup while 32 would leave CUs empty (2048 -> 2048 rank 16, the whole
+    // call on inputs from HBM: 2000 rows 40.6 us against 41.6, 4096 57.9 against 51.8,
+    // 8195 105 against 98)
     auto go = [&](auto kernel, int rows) {
       const dim3 grid(static_cast<unsigned>((a.rows + rows - 1) / rows), kRunTurns);
       hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, a);
     };
-    if (a.rows <= 4096) {
+    if (a.rows <= 2048) {
       if (a.rank <= 16) go(adapter_run_kernel<T, EVEN, 1, 1>, 16);
       else if (a.rank <= 32) go(adapter_run_kernel<T, EVEN, 1, 2>, 16);
       else go(adapter_run_kernel<T, EVEN, 1, 4>, 16);

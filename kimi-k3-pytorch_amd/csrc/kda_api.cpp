@@ -643,10 +643,14 @@ int kda_layer_decode(const kda_layer_decode_args* args, void* stream) {
 }
 
 static int check_norm(const char* what, const void* in, int64_t rows, int64_t width, double eps, int dtype,
-                      bool f64_allowed) {
+                      bool f64_allowed, int weight_is_f32) {
   g_detail[0] = '\0';
   if (!is_input_dtype(dtype) || (dtype == KDA_DTYPE_F64 && !f64_allowed)) {
     set_detail("%s: bad dtype %d", what, dtype);
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  if (weight_is_f32 && dtype == KDA_DTYPE_F64) {
+    set_detail("%s: an f32 weight beside f64", what);
     return KDA_ERR_INVALID_ARGUMENT;
   }
   if (rows <= 0 || width <= 0 || rows > INT64_MAX / 8 / width) {
@@ -664,21 +668,21 @@ static int check_norm(const char* what, const void* in, int64_t rows, int64_t wi
   return KDA_OK;
 }
 
-int kda_add_rmsnorm_fwd(const void* x, const void* residual, const void* weight, void* h, void* y, int64_t rows,
+int kda_add_rmsnorm_fwd(const void* x, const void* residual, const void* weight, int weight_is_f32, void* h, void* y, int64_t rows,
                         int64_t width, double eps, int dtype, void* stream) {
-  const int rc = check_norm("add_rmsnorm", x, rows, width, eps, dtype, true);
+  const int rc = check_norm("add_rmsnorm", x, rows, width, eps, dtype, true, weight_is_f32);
   if (rc != KDA_OK) return rc;
   if (!y || (residual && !h)) {
     set_detail("add_rmsnorm: y (and h with a residual) must be non-null");
     return KDA_ERR_INVALID_ARGUMENT;
   }
-  return launch_add_norm(x, residual, weight, h, y, nullptr, nullptr, width, rows, width, eps, dtype,
+  return launch_add_norm(x, residual, weight, weight_is_f32 != 0, h, y, nullptr, nullptr, width, rows, width, eps, dtype,
                          static_cast<hipStream_t>(stream));
 }
 
-int kda_add_rmsnorm_quant(const void* x, const void* residual, const void* weight, void* h, void* q, float* scales,
+int kda_add_rmsnorm_quant(const void* x, const void* residual, const void* weight, int weight_is_f32, void* h, void* q, float* scales,
                           int64_t group, int64_t rows, int64_t width, double eps, int dtype, void* stream) {
-  const int rc = check_norm("add_rmsnorm_quant", x, rows, width, eps, dtype, false);
+  const int rc = check_norm("add_rmsnorm_quant", x, rows, width, eps, dtype, false, weight_is_f32);
   if (rc != KDA_OK) return rc;
   if (!q || !scales || (residual && !h)) {
     set_detail("add_rmsnorm_quant: q, scales (and h with a residual) must be non-null");
@@ -690,7 +694,7 @@ int kda_add_rmsnorm_quant(const void* x, const void* residual, const void* weigh
                (long long)width, (long long)group);
     return KDA_ERR_INVALID_ARGUMENT;
   }
-  return launch_add_norm(x, residual, weight, h, nullptr, q, scales, group, rows, width, eps, dtype,
+  return launch_add_norm(x, residual, weight, weight_is_f32 != 0, h, nullptr, q, scales, group, rows, width, eps, dtype,
                          static_cast<hipStream_t>(stream));
 }
 
@@ -699,10 +703,10 @@ size_t kda_add_rmsnorm_bwd_workspace_bytes(int64_t rows, int64_t width, int dtyp
   return add_norm_bwd_workspace_bytes(rows, width, dtype);
 }
 
-int kda_add_rmsnorm_bwd(const void* h, const void* weight, const void* d_y, const void* d_h, void* dx, void* d_weight,
+int kda_add_rmsnorm_bwd(const void* h, const void* weight, int weight_is_f32, const void* d_y, const void* d_h, void* dx, void* d_weight,
                         int64_t rows, int64_t width, double eps, int dtype, void* workspace, size_t workspace_bytes,
                         void* stream) {
-  const int rc = check_norm("add_rmsnorm_bwd", h, rows, width, eps, dtype, true);
+  const int rc = check_norm("add_rmsnorm_bwd", h, rows, width, eps, dtype, true, weight_is_f32);
   if (rc != KDA_OK) return rc;
   if (!d_y || !dx) {
     set_detail("add_rmsnorm_bwd: d_y and dx must be non-null");
@@ -719,7 +723,7 @@ int kda_add_rmsnorm_bwd(const void* h, const void* weight, const void* d_y, cons
       return KDA_ERR_INVALID_ARGUMENT;
     }
   }
-  return launch_add_norm_bwd(h, weight, d_y, d_h, dx, d_weight, rows, width, eps, dtype, workspace,
+  return launch_add_norm_bwd(h, weight, weight_is_f32 != 0, d_y, d_h, dx, d_weight, rows, width, eps, dtype, workspace,
                              static_cast<hipStream_t>(stream));
 }
 

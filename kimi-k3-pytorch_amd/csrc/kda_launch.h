@@ -166,12 +166,12 @@ size_t layer_decode_workspace_bytes(const kda_layer_decode_args& d, const kda_la
 int launch_layer_decode(const kda_layer_decode_args& d, const kda_layer_adapters* ad, hipStream_t stream);
 
 // RMSNorm with the residual's addition, plain or e4m3 output (q non-null), and its backward (csrc/kda_norm.hip).
-int launch_add_norm(const void* x, const void* r, const void* w, void* h, void* y, void* q, float* scales,
+int launch_add_norm(const void* x, const void* r, const void* w, bool wide_w, void* h, void* y, void* q, float* scales,
                     int64_t group, int64_t rows, int64_t width, double eps, int dtype, hipStream_t stream);
 
 size_t add_norm_bwd_workspace_bytes(int64_t rows, int64_t width, int dtype);
 
-int launch_add_norm_bwd(const void* h, const void* w, const void* dy, const void* dh, void* dx, void* dw, int64_t rows,
+int launch_add_norm_bwd(const void* h, const void* w, bool wide_w, const void* dy, const void* dh, void* dx, void* dw, int64_t rows,
                         int64_t width, double eps, int dtype, void* workspace, hipStream_t stream);
 
 // Decode caches into and out of 8-bit pools (csrc/kda_state_pack.hip).

@@ -35,13 +35,21 @@ __device__ __forceinline__ C nan_max(C a, C b) {
 
 template <class T>
 struct AddNorm {
-  const T *x, *r, *w;  // r, w: may be null
+  const T *x, *r;      // r: may be null
+  const void* w;       // null, or of T, or (wide_w) f32
+  bool wide_w;
   T *h, *y;            // h: null without a residual (h is x)
   uint8_t* q;          // e4m3, in place of y
   float* scales;       // [rows, width / group]
   int64_t rows, width, group;
   typename NormCompute<T>::type eps;
 };
+
+template <class T>
+__device__ __forceinline__ typename NormCompute<T>::type norm_weight(const void* w, bool wide, int64_t c) {
+  if (wide) return static_cast<const float*>(w)[c];
+  return to_compute<typename NormCompute<T>::type>(static_cast<const T*>(w)[c]);
+}
 
 template <class C>
 __device__ __forceinline__ C block_sum(C v, C* part) {  // over a workgroup of four waves
@@ -77,7 +85,7 @@ __global__ __launch_bounds__(256) void add_norm_row_kernel(const AddNorm<T> a) {
   const C s = frsqrt(block_sum(ss, part) / C(D) + a.eps);
   auto value = [&](int64_t c) -> C {
     const C v = to_compute<C>(src[at + c]) * s;
-    return a.w != nullptr ? v * to_compute<C>(a.w[c]) : v;
+    return a.w != nullptr ? v * norm_weight<T>(a.w, a.wide_w, c) : v;
   };
   if constexpr (!Q) {
     for (int64_t c = tid; c < D; c += 256) a.y[at + c] = from_compute<T>(value(c));
@@ -154,6 +162,32 @@ __device__ __forceinline__ void norm_store(T* row, int i, int width, typename No
   }
 }
 
+// The weights of vector i as floats (ones without any).
+template <class T, bool FULL>
+__device__ __forceinline__ void norm_weights(const void* w, bool wide, int i, int width, float (&out)[NormVec<T>::N]) {
+  constexpr int N = NormVec<T>::N;
+  if (w == nullptr) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = 1.f;
+  } else if (!wide) {
+    typename NormVec<T>::type v{};
+    if constexpr (FULL) {
+      if (i * N < width) v = *reinterpret_cast<const typename NormVec<T>::type*>(static_cast<const T*>(w) + i * N);
+    } else {
+      v = norm_load<T, false>(static_cast<const T*>(w), i, width);
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = to_float(static_cast<T>(v[e]));
+  } else {
+#pragma unroll
+    for (int u = 0; u < N / 4; ++u) {
+      const NormVec<float>::type v = norm_load<float, FULL>(static_cast<const float*>(w), i * (N / 4) + u, width);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[4 * u + e] = v[e];
+    }
+  }
+}
+
 // Sum over the threads of a row (TPR == 64: the wave's).
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* part) {
@@ -205,19 +239,10 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void add_norm_kernel(const A
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int i = lane + j * TPR;
-    typename V::type wv{};
-    if (a.w != nullptr) {
-      if constexpr (FULL) {
-        if (i * N < width) wv = *reinterpret_cast<const typename V::type*>(a.w + i * N);
-      } else {
-        wv = norm_load<T, false>(a.w, i, width);
-      }
-    }
+    float w[N];
+    norm_weights<T, FULL>(a.w, a.wide_w, i, width, w);
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      y[j][e] = to_float(static_cast<T>(xv[j][e])) * s;
-      if (a.w != nullptr) y[j][e] *= to_float(static_cast<T>(wv[e]));
-    }
+    for (int e = 0; e < N; ++e) y[j][e] = to_float(static_cast<T>(xv[j][e])) * s * w[e];
   }
   if constexpr (!Q) {
 #pragma unroll
@@ -292,8 +317,11 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void add_norm_kernel(const A
 
 template <class T>
 struct AddNormBwd {
-  const T *h, *w, *dy, *dh;  // w, dh: may be null
-  T *dx, *dw;                // dw: may be null
+  const T *h, *dy, *dh;      // dh: may be null
+  const void* w;             // null, or of T, or (wide_w) f32; the gradient dw alike
+  bool wide_w;
+  T* dx;
+  void* dw;                  // may be null
   typename NormCompute<T>::type* s;     // [rows], for the weight gradient
   typename NormCompute<T>::type* part;  // [chunks, width] partial weight gradients
   int64_t rows, width, chunk;
@@ -308,7 +336,7 @@ __global__ __launch_bounds__(256) void add_norm_bwd_row_kernel(const AddNormBwd<
   C ss = C(0), dot = C(0);
   auto wdy = [&](int64_t c) -> C {
     const C v = to_compute<C>(a.dy[at + c]);
-    return a.w != nullptr ? v * to_compute<C>(a.w[c]) : v;
+    return a.w != nullptr ? v * norm_weight<T>(a.w, a.wide_w, c) : v;
   };
   for (int64_t c = threadIdx.x; c < D; c += 256) {
     const C h = to_compute<C>(a.h[at + c]);
@@ -338,10 +366,9 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void add_norm_bwd_kernel(con
   const int64_t group = TPR == 64 ? static_cast<int64_t>(blockIdx.x) * 4 + (tid >> 6) : blockIdx.x;
   const int64_t groups = static_cast<int64_t>(gridDim.x) * (TPR == 64 ? 4 : 1);
   float dw[NV][N] = {};
-  typename V::type wv[NV];
+  float w[NV][N];
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
-    wv[j] = a.w != nullptr ? norm_load<T, FULL>(a.w, lane + j * TPR, width) : typename V::type{};
+  for (int j = 0; j < NV; ++j) norm_weights<T, FULL>(a.w, a.wide_w, lane + j * TPR, width, w[j]);
   for (int64_t row = group; row < a.rows; row += groups) {
     const int64_t at = row * width;
     typename V::type hv[NV], yv[NV], uv[NV];
@@ -360,10 +387,8 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void add_norm_bwd_kernel(con
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const float h = to_float(static_cast<T>(hv[j][e]));
-        float g = to_float(static_cast<T>(yv[j][e]));
-        if (a.w != nullptr) g *= to_float(static_cast<T>(wv[j][e]));
         ss += h * h;
-        dot += g * h;
+        dot += to_float(static_cast<T>(yv[j][e])) * w[j][e] * h;
       }
     ss = group_sum<64>(ss);
     dot = group_sum<64>(dot);
@@ -382,8 +407,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void add_norm_bwd_kernel(con
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const float h = to_float(static_cast<T>(hv[j][e])), dy = to_float(static_cast<T>(yv[j][e]));
-        const float g = a.w != nullptr ? dy * to_float(static_cast<T>(wv[j][e])) : dy;
-        float v = s * (g - h * back);
+        float v = s * (dy * w[j][e] - h * back);
         if (a.dh != nullptr) v += to_float(static_cast<T>(uv[j][e]));
         o[e] = from_compute<T>(v);
         dw[j][e] += dy * (h * s);
@@ -448,7 +472,10 @@ __global__ __launch_bounds__(1024) void add_norm_dw_sum_kernel(const AddNormBwd<
     sum = part[0][lane];
 #pragma unroll
     for (int u = 1; u < 16; ++u) sum += part[u][lane];
-    a.dw[c] = from_compute<T>(sum);
+    if (a.wide_w)
+      static_cast<float*>(a.dw)[c] = static_cast<float>(sum);
+    else
+      static_cast<T*>(a.dw)[c] = from_compute<T>(sum);
   }
 }
 
@@ -521,10 +548,11 @@ static int run_add_norm(const AddNorm<T>& a, hipStream_t s) {
 }
 
 template <class T>
-static int add_norm_typed(const void* x, const void* r, const void* w, void* h, void* y, void* q, float* scales,
+static int add_norm_typed(const void* x, const void* r, const void* w, bool wide_w, void* h, void* y, void* q, float* scales,
                           int64_t group, int64_t rows, int64_t width, double eps, hipStream_t s) {
   AddNorm<T> a{};
-  a.x = static_cast<const T*>(x), a.r = static_cast<const T*>(r), a.w = static_cast<const T*>(w);
+  a.x = static_cast<const T*>(x), a.r = static_cast<const T*>(r), a.w = w;
+  a.wide_w = wide_w && sizeof(T) == 2;
   a.h = static_cast<T*>(h), a.y = static_cast<T*>(y), a.q = static_cast<uint8_t*>(q), a.scales = scales;
   a.rows = rows, a.width = width, a.group = group, a.eps = static_cast<typename NormCompute<T>::type>(eps);
   if constexpr (!__is_same(T, double)) {
@@ -533,17 +561,17 @@ static int add_norm_typed(const void* x, const void* r, const void* w, void* h, 
   return run_add_norm<T, false>(a, s);
 }
 
-int launch_add_norm(const void* x, const void* r, const void* w, void* h, void* y, void* q, float* scales,
+int launch_add_norm(const void* x, const void* r, const void* w, bool wide_w, void* h, void* y, void* q, float* scales,
                     int64_t group, int64_t rows, int64_t width, double eps, int dtype, hipStream_t s) {
   if (!grid_fits(rows)) {
     set_detail("add_rmsnorm: %lld rows", (long long)rows);
     return KDA_ERR_UNSUPPORTED;
   }
   switch (dtype) {
-    case KDA_DTYPE_BF16: return add_norm_typed<bf16>(x, r, w, h, y, q, scales, group, rows, width, eps, s);
-    case KDA_DTYPE_F16: return add_norm_typed<f16>(x, r, w, h, y, q, scales, group, rows, width, eps, s);
-    case KDA_DTYPE_F32: return add_norm_typed<float>(x, r, w, h, y, q, scales, group, rows, width, eps, s);
-    default: return add_norm_typed<double>(x, r, w, h, y, q, scales, group, rows, width, eps, s);
+    case KDA_DTYPE_BF16: return add_norm_typed<bf16>(x, r, w, wide_w, h, y, q, scales, group, rows, width, eps, s);
+    case KDA_DTYPE_F16: return add_norm_typed<f16>(x, r, w, wide_w, h, y, q, scales, group, rows, width, eps, s);
+    case KDA_DTYPE_F32: return add_norm_typed<float>(x, r, w, wide_w, h, y, q, scales, group, rows, width, eps, s);
+    default: return add_norm_typed<double>(x, r, w, wide_w, h, y, q, scales, group, rows, width, eps, s);
   }
 }
 
@@ -590,12 +618,12 @@ static void launch_bwd_rows(const AddNormBwd<T>& a, RowShape r, int64_t blocks, 
 }
 
 template <class T>
-static int add_norm_bwd_typed(const void* h, const void* w, const void* dy, const void* dh, void* dx, void* dw,
+static int add_norm_bwd_typed(const void* h, const void* w, bool wide_w, const void* dy, const void* dh, void* dx, void* dw,
                               int64_t rows, int64_t width, double eps, void* ws, hipStream_t s) {
   using C = typename NormCompute<T>::type;
   AddNormBwd<T> a{};
-  a.h = static_cast<const T*>(h), a.w = static_cast<const T*>(w), a.dy = static_cast<const T*>(dy);
-  a.dh = static_cast<const T*>(dh), a.dx = static_cast<T*>(dx), a.dw = static_cast<T*>(dw);
+  a.h = static_cast<const T*>(h), a.w = w, a.wide_w = wide_w && sizeof(T) == 2, a.dy = static_cast<const T*>(dy);
+  a.dh = static_cast<const T*>(dh), a.dx = static_cast<T*>(dx), a.dw = dw;
   a.rows = rows, a.width = width, a.eps = static_cast<C>(eps);
   const RowShape r = row_shape(width, sizeof(T), rows);
   const DwPlan p = dw_plan(rows, width, sizeof(T));
@@ -617,17 +645,17 @@ static int add_norm_bwd_typed(const void* h, const void* w, const void* dy, cons
   return check_launch("add_norm_bwd");
 }
 
-int launch_add_norm_bwd(const void* h, const void* w, const void* dy, const void* dh, void* dx, void* dw, int64_t rows,
+int launch_add_norm_bwd(const void* h, const void* w, bool wide_w, const void* dy, const void* dh, void* dx, void* dw, int64_t rows,
                         int64_t width, double eps, int dtype, void* ws, hipStream_t s) {
   if (!grid_fits(rows)) {
     set_detail("add_rmsnorm_bwd: %lld rows", (long long)rows);
     return KDA_ERR_UNSUPPORTED;
   }
   switch (dtype) {
-    case KDA_DTYPE_BF16: return add_norm_bwd_typed<bf16>(h, w, dy, dh, dx, dw, rows, width, eps, ws, s);
-    case KDA_DTYPE_F16: return add_norm_bwd_typed<f16>(h, w, dy, dh, dx, dw, rows, width, eps, ws, s);
-    case KDA_DTYPE_F32: return add_norm_bwd_typed<float>(h, w, dy, dh, dx, dw, rows, width, eps, ws, s);
-    default: return add_norm_bwd_typed<double>(h, w, dy, dh, dx, dw, rows, width, eps, ws, s);
+    case KDA_DTYPE_BF16: return add_norm_bwd_typed<bf16>(h, w, wide_w, dy, dh, dx, dw, rows, width, eps, ws, s);
+    case KDA_DTYPE_F16: return add_norm_bwd_typed<f16>(h, w, wide_w, dy, dh, dx, dw, rows, width, eps, ws, s);
+    case KDA_DTYPE_F32: return add_norm_bwd_typed<float>(h, w, wide_w, dy, dh, dx, dw, rows, width, eps, ws, s);
+    default: return add_norm_bwd_typed<double>(h, w, wide_w, dy, dh, dx, dw, rows, width, eps, ws, s);
   }
 }
 

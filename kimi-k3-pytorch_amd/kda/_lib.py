@@ -143,10 +143,10 @@ SIGNATURES = {
     "kda_adapter_linear_takes_weight": (_I, [_P]),
     "kda_adapter_linear_workspace_bytes": (_S, [_P]),
     "kda_adapter_linear": (_I, [_P, _P]),
-    "kda_add_rmsnorm_fwd": (_I, [_P] * 5 + [_L, _L, ctypes.c_double, _I, _P]),
-    "kda_add_rmsnorm_quant": (_I, [_P] * 6 + [_L, _L, _L, ctypes.c_double, _I, _P]),
+    "kda_add_rmsnorm_fwd": (_I, [_P] * 3 + [_I, _P, _P, _L, _L, ctypes.c_double, _I, _P]),
+    "kda_add_rmsnorm_quant": (_I, [_P] * 3 + [_I] + [_P] * 3 + [_L, _L, _L, ctypes.c_double, _I, _P]),
     "kda_add_rmsnorm_bwd_workspace_bytes": (_S, [_L, _L, _I]),
-    "kda_add_rmsnorm_bwd": (_I, [_P] * 6 + [_L, _L, ctypes.c_double, _I, _P, _S, _P]),
+    "kda_add_rmsnorm_bwd": (_I, [_P, _P, _I] + [_P] * 4 + [_L, _L, ctypes.c_double, _I, _P, _S, _P]),
 }
 
 _lock = threading.Lock()

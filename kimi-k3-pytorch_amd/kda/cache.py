@@ -384,7 +384,7 @@ def pack_states(states: Sequence[KDAState], *, out: Sequence[PackedKDAState] | N
             moves.append(_pack(src[0], out[i].recurrent))
             moves += [_bytes(a, b) for a, b in zip(src[1:], dst[1:])]
             size += src[0].numel() * 4
-            if size >= LAUNCH_BYTES or i + 1 == len(layers):
+            if size >= LAUNCH_BYTES or len(moves) >= 60 or i + 1 == len(layers):
                 _move(moves, code, None, batch, slots, entries, batch, status, stream)
                 moves, size = [], 0
         _check_slots(status, entries)
@@ -423,7 +423,7 @@ def unpack_states(packed: Sequence[PackedKDAState], slots: torch.Tensor | None =
             moves += [_bytes(a, b) for a, b in zip(rest, new[1:])]
             waiting.append(new)
             size += new[0].numel() * 4
-            if size >= LAUNCH_BYTES or i + 1 == len(packed):
+            if size >= LAUNCH_BYTES or len(moves) >= 60 or i + 1 == len(packed):
                 _move(moves, code, slots, entries, None, n, n, status, stream)
                 states += [_rebuild(x) for x in waiting]
                 moves, size, waiting = [], 0, []

@@ -591,7 +591,8 @@ def _check_add_norm(x, residual, weight, eps, dtypes) -> None:
     if weight is not None:
         if weight.shape != (x.shape[-1],):
             raise ValueError(f"weight must have shape [{x.shape[-1]}], got {tuple(weight.shape)}")
-        _check_dtype("weight", weight, x.dtype)
+        if weight.dtype != x.dtype and (weight.dtype != torch.float32 or x.dtype == torch.float64):
+            raise TypeError(f"weight must have dtype {x.dtype} or float32, got {weight.dtype}")
         _check_device("weight", weight, x.device)
     if not eps > 0:
         raise ValueError("eps must be > 0")
@@ -607,7 +608,7 @@ def add_rmsnorm(
     """``(y, h)``: the sum ``h = x + residual`` of ``[..., D]`` tensors of one dtype
     (``h`` is ``x`` itself without a residual) and its RMSNorm
     ``y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension, ``weight [D]``
-    or None.  The norm reads the sum as it is stored, rounded to the dtype.
+    (of that dtype, or f32) or None.  The norm reads the sum as it is stored, rounded to the dtype.
     Differentiable in all tensors (``kda_add_rmsnorm_bwd``; the weight gradient
     is summed in a fixed order)."""
     _check_add_norm(x, residual, weight, eps, _DTYPES)
@@ -616,6 +617,11 @@ def add_rmsnorm(
     else:
         y, h = _add_norm_forward(x, residual, weight, float(eps))
     return y, (x if residual is None else h)
+
+
+def _f32(weight, x) -> int:
+    """Whether a weight is f32 beside 16-bit tensors (a mixed-precision model's)."""
+    return 1 if weight is not None and weight.dtype != x.dtype else 0
 
 
 def _add_norm_forward(x, residual, weight, eps):
@@ -627,8 +633,8 @@ def _add_norm_forward(x, residual, weight, eps):
         wc = None if weight is None else weight.contiguous()
         with _prep.on_device(x.device):
             _lib.check(_lib.load().kda_add_rmsnorm_fwd(
-                xc.data_ptr(), _lib.ptr(rc), _lib.ptr(wc), _lib.ptr(h), y.data_ptr(), xc.numel() // x.shape[-1],
-                x.shape[-1], eps, _lib.dtype_code(x.dtype), _prep.stream(x.device)))
+                xc.data_ptr(), _lib.ptr(rc), _lib.ptr(wc), _f32(wc, x), _lib.ptr(h), y.data_ptr(),
+                xc.numel() // x.shape[-1], x.shape[-1], eps, _lib.dtype_code(x.dtype), _prep.stream(x.device)))
     return y, h
 
 
@@ -662,7 +668,7 @@ class _AddRMSNorm(torch.autograd.Function):
                 nbytes = lib.kda_add_rmsnorm_bwd_workspace_bytes(rows, width, code) if need_w else 0
                 workspace = _prep.workspace(nbytes, h.device, "the add_rmsnorm backward")
                 _lib.check(lib.kda_add_rmsnorm_bwd(
-                    hc.data_ptr(), _lib.ptr(wc), dyc.data_ptr(), _lib.ptr(dhc), dx.data_ptr(), _lib.ptr(dw), rows,
+                    hc.data_ptr(), _lib.ptr(wc), _f32(wc, h), dyc.data_ptr(), _lib.ptr(dhc), dx.data_ptr(), _lib.ptr(dw), rows,
                     width, ctx.eps, code, _lib.ptr(workspace), nbytes, _prep.stream(h.device)))
         return dx if need_x else None, dx if need_r else None, dw, None
 
@@ -702,8 +708,8 @@ def add_rmsnorm_quant(
         wc = None if weight is None else weight.contiguous()
         with _prep.on_device(x.device):
             _lib.check(_lib.load().kda_add_rmsnorm_quant(
-                xc.data_ptr(), _lib.ptr(rc), _lib.ptr(wc), _lib.ptr(h), q.data_ptr(), scales.data_ptr(), group,
-                xc.numel() // width, width, float(eps), _lib.dtype_code(x.dtype), _prep.stream(x.device)))
+                xc.data_ptr(), _lib.ptr(rc), _lib.ptr(wc), _f32(wc, x), _lib.ptr(h), q.data_ptr(), scales.data_ptr(),
+                group, xc.numel() // width, width, float(eps), _lib.dtype_code(x.dtype), _prep.stream(x.device)))
     return q, scales, (x if residual is None else h)
 
 

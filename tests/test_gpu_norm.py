@@ -91,6 +91,33 @@ def test_add_rmsnorm_gradients_against_differences():
     assert torch.autograd.gradcheck(lambda a, b: fused.add_rmsnorm(a, b, None), leaves[:2])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,width", [(3, 7), (40, 512), (9, 1001), (5, 7168), (1500, 264), (2, 40000)])
+def test_a_weight_in_f32_beside_16_bit_tensors(rows, width, dtype):
+    x, r, _ = _inputs(rows, width, dtype)
+    w = _rand(width, dtype=torch.float32, seed=9, scale=0.1, mean=1.0)
+    dy = _rand(rows, width, dtype=dtype, seed=5)
+    leaves = [t.to(DEV).requires_grad_() for t in (x, r, w)]
+    y, h = fused.add_rmsnorm(*leaves)
+    got = torch.autograd.grad(y, leaves, dy.to(DEV))
+    ref, hs = ora.add_rmsnorm(x, r, w)
+    assert y.dtype == dtype and got[2].dtype == torch.float32
+    assert_within(y, ref, rounded(ref, dtype) + ref.abs() * _units(width, dtype), "y")
+    dx, dw = ora.add_rmsnorm_backward(hs, w, dy, None)
+    hd, wdy = hs.double(), dy.double() * w.double()
+    s = 1 / torch.sqrt(hd.square().mean(-1, keepdim=True) + 1e-6)
+    terms = s * wdy.abs() + hd.abs() * s ** 3 * (wdy * hd).abs().mean(-1, keepdim=True)
+    for t in got[:2]:
+        assert_within(t, dx, rounded(dx, dtype) + 3 * _units(width, dtype) * terms, "dx")
+    sums = (dy.double() * hd * s).abs().sum(0)
+    assert_within(got[2], dw, (rows / 64 + 68 + width / 512 + 16) * 2.0 ** -24 * sums, "dw")
+    with torch.no_grad():
+        q, scales, _ = fused.add_rmsnorm_quant(*leaves)
+    quotients, ref_scales = ora.e4m3_groups(ref, width)
+    assert_within(scales, ref_scales, ref_scales * (_units(width, dtype) + 2.0 ** -23), "scales")
+    assert float((q.float().cpu() - quotients).abs().max()) <= 448 * 2.0 ** -4 * 1.1
+
+
 def test_gradients_of_inputs_that_are_used_twice_and_partly():
     # the sum is its own residual, and only one of the outputs is used
     x = _rand(4, 96, dtype=torch.float64, seed=3).to(DEV).requires_grad_()

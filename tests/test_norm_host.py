@@ -25,6 +25,8 @@ def test_argument_checks(call):
     with pytest.raises(TypeError):
         call(x, x, torch.zeros(64, dtype=torch.bfloat16))
     with pytest.raises(TypeError):
+        call(x.half(), x.half(), torch.zeros(64, dtype=torch.bfloat16))
+    with pytest.raises(TypeError):
         call(torch.zeros(3, 64, dtype=torch.int32))
     for eps in (0.0, -1.0, float("nan")):
         with pytest.raises(ValueError):
@@ -45,16 +47,16 @@ def test_entry_points_reject_bad_arguments():
     lib = _lib.load()
     a, bad = 4096, _lib.KDA_ERR_INVALID_ARGUMENT
 
-    def fwd(x=a, r=a, h=a, y=a, rows=4, width=64, eps=1e-6, dtype=2):
-        return lib.kda_add_rmsnorm_fwd(x, r, a, h, y, rows, width, eps, dtype, None)
+    def fwd(x=a, r=a, h=a, y=a, f32=0, rows=4, width=64, eps=1e-6, dtype=2):
+        return lib.kda_add_rmsnorm_fwd(x, r, a, f32, h, y, rows, width, eps, dtype, None)
 
     for kw in (dict(x=None), dict(y=None), dict(h=None), dict(rows=0), dict(width=0), dict(width=-1), dict(eps=0.0),
-               dict(dtype=9), dict(rows=1 << 40, width=1 << 40)):
+               dict(dtype=9), dict(dtype=3, f32=1), dict(rows=1 << 40, width=1 << 40)):
         assert fwd(**kw) == bad, kw
     assert fwd(rows=1 << 31) == _lib.KDA_ERR_UNSUPPORTED
 
     def quant(group, width=192, dtype=2, q=a):
-        return lib.kda_add_rmsnorm_quant(a, None, None, None, q, a, group, 4, width, 1e-6, dtype, None)
+        return lib.kda_add_rmsnorm_quant(a, None, None, 0, None, q, a, group, 4, width, 1e-6, dtype, None)
 
     for kw in (dict(group=128), dict(group=16), dict(group=0), dict(group=64, dtype=3), dict(group=64, q=None)):
         assert quant(**kw) == bad, kw
@@ -63,7 +65,7 @@ def test_entry_points_reject_bad_arguments():
     assert need > 0 and lib.kda_add_rmsnorm_bwd_workspace_bytes(0, 64, 2) == 0
 
     def bwd(ws=a, nbytes=need, dy=a, dw=a):
-        return lib.kda_add_rmsnorm_bwd(a, a, dy, None, a, dw, 100, 64, 1e-6, 2, ws, nbytes, None)
+        return lib.kda_add_rmsnorm_bwd(a, a, 0, dy, None, a, dw, 100, 64, 1e-6, 2, ws, nbytes, None)
 
     assert bwd(ws=None) == _lib.KDA_ERR_WORKSPACE and bwd(nbytes=need - 1) == _lib.KDA_ERR_WORKSPACE
     assert bwd(ws=a + 4) == bad and bwd(dy=None) == bad
