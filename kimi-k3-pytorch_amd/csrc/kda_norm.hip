@@ -162,6 +162,18 @@ __device__ __forceinline__ void norm_store(T* row, int i, int width, typename No
   }
 }
 
+// A weight's vector: read by every row, so no streaming load.
+template <class T, bool FULL>
+__device__ __forceinline__ typename NormVec<T>::type weight_load(const T* w, int i, int width) {
+  if constexpr (FULL) {
+    typename NormVec<T>::type v{};
+    if (i * NormVec<T>::N < width) v = *reinterpret_cast<const typename NormVec<T>::type*>(w + i * NormVec<T>::N);
+    return v;
+  } else {
+    return norm_load<T, false>(w, i, width);
+  }
+}
+
 // The weights of vector i as floats (ones without any).
 template <class T, bool FULL>
 __device__ __forceinline__ void norm_weights(const void* w, bool wide, int i, int width, float (&out)[NormVec<T>::N]) {
@@ -170,18 +182,13 @@ __device__ __forceinline__ void norm_weights(const void* w, bool wide, int i, in
 #pragma unroll
     for (int e = 0; e < N; ++e) out[e] = 1.f;
   } else if (!wide) {
-    typename NormVec<T>::type v{};
-    if constexpr (FULL) {
-      if (i * N < width) v = *reinterpret_cast<const typename NormVec<T>::type*>(static_cast<const T*>(w) + i * N);
-    } else {
-      v = norm_load<T, false>(static_cast<const T*>(w), i, width);
-    }
+    const typename NormVec<T>::type v = weight_load<T, FULL>(static_cast<const T*>(w), i, width);
 #pragma unroll
     for (int e = 0; e < N; ++e) out[e] = to_float(static_cast<T>(v[e]));
   } else {
 #pragma unroll
     for (int u = 0; u < N / 4; ++u) {
-      const NormVec<float>::type v = norm_load<float, FULL>(static_cast<const float*>(w), i * (N / 4) + u, width);
+      const NormVec<float>::type v = weight_load<float, FULL>(static_cast<const float*>(w), i * (N / 4) + u, width);
 #pragma unroll
       for (int e = 0; e < 4; ++e) out[4 * u + e] = v[e];
     }
@@ -215,6 +222,11 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void add_norm_kernel(const A
   typename V::type xv[NV], rv[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) xv[j] = norm_load<T, FULL>(a.x + at, lane + j * TPR, width);
+  typename V::type wv[NV];  // asked for ahead of the sum
+  if (a.w != nullptr && !a.wide_w) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) wv[j] = weight_load<T, FULL>(static_cast<const T*>(a.w), lane + j * TPR, width);
+  }
   float ss = 0.f;
   if (a.r != nullptr) {
 #pragma unroll
@@ -239,10 +251,17 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void add_norm_kernel(const A
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int i = lane + j * TPR;
-    float w[N];
-    norm_weights<T, FULL>(a.w, a.wide_w, i, width, w);
 #pragma unroll
-    for (int e = 0; e < N; ++e) y[j][e] = to_float(static_cast<T>(xv[j][e])) * s * w[e];
+    for (int e = 0; e < N; ++e) y[j][e] = to_float(static_cast<T>(xv[j][e])) * s;
+    if (a.w != nullptr && !a.wide_w) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) y[j][e] *= to_float(static_cast<T>(wv[j][e]));
+    } else if (a.w != nullptr) {
+      float w[N];
+      norm_weights<T, FULL>(a.w, true, i, width, w);
+#pragma unroll
+      for (int e = 0; e < N; ++e) y[j][e] *= w[e];
+    }
   }
   if constexpr (!Q) {
 #pragma unroll
