@@ -15,7 +15,10 @@ namespace kda {
 
 constexpr int kMoveMax = 64;  // tensors per launch
 constexpr int kMoveThreads = 256;
-constexpr int kMoveSteps = 4;  // loads of a thread in flight
+// Loads of a thread in flight.  8 layers x 32 sequences x 32 heads, 128 x 128: packing
+// 146 us with 8 and 154 with 4, reading back 141 and 132 (2: 195 and 163).
+constexpr int kPackSteps = 8;
+constexpr int kMoveSteps = 4;
 constexpr float kTinyRow = 0x1p-100f;
 
 struct Move {
@@ -56,20 +59,63 @@ __device__ __forceinline__ int quotient(float x, float s, float inv) {
 struct RowScale {
   float scale, inv;
 };
-__device__ __forceinline__ RowScale row_scale(float top) {
-  if (!(top <= 3.402823466e38f)) return {__builtin_nanf(""), 0.f};
+// of a row's largest magnitude, as its bits
+__device__ __forceinline__ RowScale row_scale(unsigned bits) {
+  const float top = __builtin_bit_cast(float, bits);
+  if (bits >= 0x7f800000u) return {__builtin_nanf(""), 0.f};
   if (top < kTinyRow) return {0.f, 0.f};
   const float s = top * (1.f / 127.f);
   return {s, frcp(s)};
 }
-// the quotient, zeros for rows without a scale
-__device__ __forceinline__ int packed_value(float x, const RowScale& r) {
-  return r.inv != 0.f ? quotient(x, r.scale, r.inv) : 0;
+
+// Four quotients as bytes, zeros for rows without a scale.  x inv + 1.5 2^23 holds the
+// nearest whole number n in its low bits; x inv is off by 127 2^-23 at most, so n is
+// the exact quotient's unless x inv lies within 2e-5 of a tie, where the residual
+// decides.  (Deciding so for every value takes 14 instructions each, which bound
+// the kernel: 154 us against the 127 that its bytes take at the copy's rate.)
+__device__ __forceinline__ unsigned packed_four(const float (&x)[4], const RowScale& r) {
+  constexpr float kWhole = 12582912.f;
+  float n[4];
+  bool near = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    n[e] = fmaf(x[e], r.inv, kWhole);
+    near |= fabsf(fmaf(x[e], r.inv, -(n[e] - kWhole))) > 0.49998f;
+  }
+  unsigned b[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) b[e] = __builtin_bit_cast(unsigned, n[e]);
+  if (__ballot(near) != 0) {  // about one wave in a hundred
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (r.inv != 0.f) b[e] = static_cast<unsigned>(quotient(x[e], r.scale, r.inv));
+  }
+  // the low bytes of the four
+  const unsigned lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u);
+  return r.inv != 0.f ? lo | hi << 16 : 0u;
 }
 
-__device__ __forceinline__ float abs_max(float a, float b) {  // of magnitudes, a NaN if either is
-  a = fabsf(a);
-  return (a > b || a != a) ? a : b;
+// The larger one of magnitudes' bits: as numbers, infinity over all, NaN over infinity.
+__device__ __forceinline__ unsigned top_bits(float x, unsigned top) {
+  const unsigned b = __builtin_bit_cast(unsigned, x) & 0x7fffffffu;
+  return b > top ? b : top;
+}
+template <int ctrl>
+__device__ __forceinline__ unsigned dpp_max(unsigned v) {
+  const unsigned o = static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), ctrl, 0xf, 0xf, false));
+  return o > v ? o : v;
+}
+// over `lanes` neighbouring lanes (a power of two, the same in every lane)
+__device__ __forceinline__ unsigned group_top(unsigned v, int lanes) {
+  if (lanes >= 2) v = dpp_max<0xb1>(v);    // the moves of group_sum
+  if (lanes >= 4) v = dpp_max<0x4e>(v);
+  if (lanes >= 8) v = dpp_max<0x141>(v);
+  if (lanes >= 16) v = dpp_max<0x140>(v);
+  for (int off = 16; off < lanes; off <<= 1) {
+    const unsigned o = __shfl_xor(v, off);
+    v = o > v ? o : v;
+  }
+  return v;
 }
 
 typedef int8_t char4_t __attribute__((ext_vector_type(4)));
@@ -79,66 +125,70 @@ struct Four {
   typedef T type __attribute__((ext_vector_type(4)));
 };
 
-template <class T>
-__device__ __forceinline__ void pack_tile(const Move& d, int64_t from, int64_t to, int64_t row0, bool write) {
+// `place()` finds the destination entry, -1 for none; every thread calls it, once,
+// after the rows' loads have been asked for: its own loads and its barrier take as
+// long again.
+template <class T, class F>
+__device__ __forceinline__ void pack_tile(const Move& d, int64_t from, int64_t row0, F place) {
   const T* src = static_cast<const T*>(d.src) + from * d.rows * d.width;
-  int8_t* dst = static_cast<int8_t*>(d.dst) + to * d.rows * d.width;
-  float* scales = d.scales + to * d.rows;
   const int tid = threadIdx.x;
   if (d.lanes != 0) {
     typedef typename Four<T>::type v4;
     const int c = 4 * (tid % d.lanes), step = kMoveThreads / d.lanes;
     const int64_t first = row0 + tid / d.lanes;
-    float x[kMoveSteps][4];
+    v4 x[kPackSteps];
 #pragma unroll
-    for (int u = 0; u < kMoveSteps; ++u) {
+    for (int u = 0; u < kPackSteps; ++u) {
       const int64_t row = first + u * step;
-      v4 v{};
+      x[u] = v4{};
       if (row < d.rows && c < d.width)
-        v = __builtin_nontemporal_load(reinterpret_cast<const v4*>(src + row * d.width + c));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[u][e] = to_float(static_cast<T>(v[e]));
+        x[u] = __builtin_nontemporal_load(reinterpret_cast<const v4*>(src + row * d.width + c));
     }
+    const int64_t to = place();
+    if (to < 0) return;  // the whole workgroup
+    int8_t* dst = static_cast<int8_t*>(d.dst) + to * d.rows * d.width;
+    float* scales = d.scales + to * d.rows;
 #pragma unroll
-    for (int u = 0; u < kMoveSteps; ++u) {
-      float top = 0.f;
+    for (int u = 0; u < kPackSteps; ++u) {
+      float v[4];
+      unsigned top = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) top = abs_max(x[u][e], top);
-      for (int off = 1; off < d.lanes; off <<= 1) top = abs_max(__shfl_xor(top, off), top);
-      const RowScale r = row_scale(top);
+      for (int e = 0; e < 4; ++e) {
+        v[e] = to_float(static_cast<T>(x[u][e]));
+        top = top_bits(v[e], top);
+      }
+      const RowScale r = row_scale(group_top(top, d.lanes));
+      const unsigned q = packed_four(v, r);
       const int64_t row = first + u * step;
-      if (!write || row >= d.rows || c >= d.width) continue;
-      char4_t q;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) q[e] = static_cast<int8_t>(packed_value(x[u][e], r));
-      __builtin_nontemporal_store(q, reinterpret_cast<char4_t*>(dst + row * d.width + c));
+      if (row >= d.rows || c >= d.width) continue;
+      __builtin_nontemporal_store(q, reinterpret_cast<unsigned*>(dst + row * d.width + c));
       if (c == 0) scales[row] = r.scale;
     }
-  } else if (write) {
-    const int lane = tid & 63;
-    for (int64_t row = row0 + (tid >> 6); row < row0 + d.tile_rows && row < d.rows; row += kMoveThreads / 64) {
-      const T* p = src + row * d.width;
-      float top = 0.f;
-      for (int c = lane; c < d.width; c += 64) top = abs_max(to_float(p[c]), top);
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) top = abs_max(__shfl_xor(top, off), top);
-      const RowScale r = row_scale(top);
-      for (int c = lane; c < d.width; c += 64)
-        dst[row * d.width + c] = static_cast<int8_t>(packed_value(to_float(p[c]), r));
-      if (lane == 0) scales[row] = r.scale;
-    }
+    return;
+  }
+  const int64_t to = place();
+  if (to < 0) return;
+  int8_t* dst = static_cast<int8_t*>(d.dst) + to * d.rows * d.width;
+  float* scales = d.scales + to * d.rows;
+  const int lane = tid & 63;
+  for (int64_t row = row0 + (tid >> 6); row < row0 + d.tile_rows && row < d.rows; row += kMoveThreads / 64) {
+    const T* p = src + row * d.width;
+    unsigned top = 0;
+    for (int c = lane; c < d.width; c += 64) top = top_bits(to_float(p[c]), top);
+    const RowScale r = row_scale(group_top(top, 64));
+    for (int c = lane; c < d.width; c += 64)
+      dst[row * d.width + c] = static_cast<int8_t>(r.inv != 0.f ? quotient(to_float(p[c]), r.scale, r.inv) : 0);
+    if (lane == 0) scales[row] = r.scale;
   }
 }
 
 // `there`: whether the source slot exists; its rows are NaN otherwise
 template <class T>
-__device__ __forceinline__ void unpack_tile(const Move& d, int64_t from, int64_t to, int64_t row0, bool there,
-                                            bool write) {
+__device__ __forceinline__ void unpack_tile(const Move& d, int64_t from, int64_t to, int64_t row0, bool there) {
   const int8_t* src = static_cast<const int8_t*>(d.src) + (there ? from : 0) * d.rows * d.width;
   const float* scales = d.scales + (there ? from : 0) * d.rows;
   T* dst = static_cast<T*>(d.dst) + to * d.rows * d.width;
   const int tid = threadIdx.x;
-  if (!write) return;
   if (d.lanes != 0) {
     typedef typename Four<T>::type v4;
     const int c = 4 * (tid % d.lanes), step = kMoveThreads / d.lanes;
@@ -174,11 +224,9 @@ __device__ __forceinline__ void unpack_tile(const Move& d, int64_t from, int64_t
 }
 
 template <class U>
-__device__ __forceinline__ void copy_tile(const Move& d, int64_t from, int64_t to, int64_t tile, bool there,
-                                          bool write) {
+__device__ __forceinline__ void copy_tile(const Move& d, int64_t from, int64_t to, int64_t tile, bool there) {
   const U* src = static_cast<const U*>(d.src) + (there ? from : 0) * d.width;
   U* dst = static_cast<U*>(d.dst) + to * d.width;
-  if (!write) return;
   const int64_t c0 = tile * kMoveThreads * kMoveSteps + threadIdx.x;
 #pragma unroll
   for (int u = 0; u < kMoveSteps; ++u) {
@@ -200,40 +248,49 @@ __global__ __launch_bounds__(kMoveThreads) void state_move_kernel(const MoveArgs
       hi = mid - 1;
   }
   const Move& d = a.d[lo];
-  const int64_t i = (block - d.tile0) / d.tiles, tile = (block - d.tile0) % d.tiles;
-  const int64_t from = a.src_index != nullptr ? a.src_index[i] : i, to = a.dst_index != nullptr ? a.dst_index[i] : i;
+  const unsigned at = static_cast<unsigned>(block - d.tile0), tiles = static_cast<unsigned>(d.tiles);  // below 2^31
+  const int64_t i = at / tiles, tile = at % tiles;
+  const int64_t from = a.src_index != nullptr ? a.src_index[i] : i;
   const bool there = from >= 0 && from < a.n_src;
-  bool write = to >= 0 && to < a.n_dst;
-  if ((!there || !write) && threadIdx.x == 0 && a.status != nullptr) *a.status = 1;
-  if (a.dst_index != nullptr) {  // a slot that is named twice takes its last entry
-    int later = 0;
-    for (int64_t j = i + 1 + threadIdx.x; j < a.n; j += kMoveThreads) later |= a.dst_index[j] == to;
-    if (__syncthreads_or(later)) write = false;
+  if (!there && threadIdx.x == 0 && a.status != nullptr) *a.status = 1;
+  auto place = [&]() -> int64_t {
+    const int64_t to = a.dst_index != nullptr ? a.dst_index[i] : i;
+    const bool fits = to >= 0 && to < a.n_dst;
+    if (!fits && threadIdx.x == 0 && a.status != nullptr) *a.status = 1;
+    if (a.dst_index != nullptr) {  // a slot that is named twice takes its last entry
+      int later = 0;
+      for (int64_t j = i + 1 + threadIdx.x; j < a.n; j += kMoveThreads) later |= a.dst_index[j] == to;
+      if (__syncthreads_or(later)) return -1;
+    }
+    return fits ? to : -1;
+  };
+  if (d.kind == KDA_MOVE_PACK) {
+    if (there) pack_tile<T>(d, from, tile * d.tile_rows, place);
+    return;
   }
+  const int64_t to = place();
+  if (to < 0) return;
   switch (d.kind) {
-    case KDA_MOVE_PACK:
-      pack_tile<T>(d, there ? from : 0, to, tile * d.tile_rows, write && there);
-      break;
     case KDA_MOVE_UNPACK:
-      unpack_tile<T>(d, from, to, tile * d.tile_rows, there, write);
+      unpack_tile<T>(d, from, to, tile * d.tile_rows, there);
       break;
     default:
       switch (d.lanes) {
         case 4:
           typedef unsigned u4 __attribute__((ext_vector_type(4)));
-          copy_tile<u4>(d, from, to, tile, there, write);
+          copy_tile<u4>(d, from, to, tile, there);
           break;
         case 3:
-          copy_tile<uint64_t>(d, from, to, tile, there, write);
+          copy_tile<uint64_t>(d, from, to, tile, there);
           break;
         case 2:
-          copy_tile<uint32_t>(d, from, to, tile, there, write);
+          copy_tile<uint32_t>(d, from, to, tile, there);
           break;
         case 1:
-          copy_tile<uint16_t>(d, from, to, tile, there, write);
+          copy_tile<uint16_t>(d, from, to, tile, there);
           break;
         default:
-          copy_tile<uint8_t>(d, from, to, tile, there, write);
+          copy_tile<uint8_t>(d, from, to, tile, there);
           break;
       }
   }
@@ -361,7 +418,7 @@ int launch_state_move(const kda_state_tensor* t, int count, int dtype, const int
       if (d.width % 4 == 0 && d.width <= 256 && wide % (4 * float_bytes(dtype)) == 0 && narrow % 4 == 0)
         for (lanes = 1; lanes * 4 < d.width;) lanes *= 2;
       d.lanes = static_cast<int16_t>(lanes);
-      d.tile_rows = lanes != 0 ? kMoveThreads / lanes * kMoveSteps : kMoveThreads / 64 * kMoveSteps;
+      d.tile_rows = kMoveThreads / (lanes != 0 ? lanes : 64) * (pack ? kPackSteps : kMoveSteps);
       per = (d.rows + d.tile_rows - 1) / d.tile_rows;
     }
     if (per > 0x7fffffffLL / n) {
