@@ -253,7 +253,8 @@ struct LowRows {  // s of R rows, RANK of the rank
   __device__ __forceinline__ void put(int r, int j, float v) {
     const U hi = static_cast<U>(v);
     s[0][r][j] = hi;
-    if constexpr (P == 2) s[P - 1][r][j] = static_cast<U>(v - static_cast<float>(hi));
+    const float f = static_cast<float>(hi);
+    if constexpr (P == 2) s[P - 1][r][j] = static_cast<U>(v == f ? 0.f : v - f);  // nothing is left of an infinity
   }
 };
 

@@ -114,6 +114,21 @@ def test_rows_are_independent(batch, tokens, dtype):
     assert bool(got[~good].isnan().all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,tokens", [(6, 1), (60, 1), (6, 40)])
+def test_infinities_stay_infinities(batch, tokens, dtype):
+    # one infinite input, rank 1: every product of its row is an infinity of some sign
+    x, w, bias, a, b, scaling, _ = _inputs(batch, tokens, 64, 64, 1, 3, dtype)
+    ids = torch.arange(batch) % 3
+    x[2, 0, 5] = float("inf")
+    x[4, 0, 7] = float("-inf")
+    got = _call(x, w, bias, a, b, scaling, ids).cpu().reshape(-1, 64)
+    y, _, _ = ora.adapter_linear(x.reshape(-1, 64), w, bias, a, b, scaling, ids.repeat_interleave(tokens))
+    assert bool(y.isinf().any())
+    assert torch.equal(got.isnan(), y.isnan()) and torch.equal(got.isinf(), y.isinf())
+    assert torch.equal(got[y.isinf()].sign().double(), y[y.isinf()].sign())
+
+
 def test_layouts():
     x, w, bias, a, b, scaling, ids = _dev(*_inputs(6, 3, 96, 40, 8, 4, torch.bfloat16))
     stack = adapters.AdapterStack(a, b, scaling)
