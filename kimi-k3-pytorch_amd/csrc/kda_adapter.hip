@@ -6,7 +6,7 @@
 // First s_m = A_a x_m in f32 (down), then c_a B_a s_m (up).  Rows that share an
 // adapter share its reading; whose rows they are is found by the kernels
 // themselves, so a call needs no sorted batch and no plan:
-//  - runs (a prompt's tokens): a workgroup owns 32 neighbouring rows and goes through
+//  - runs (a prompt's tokens): a workgroup owns 16 or 32 neighbouring rows and goes through
 //    the adapters it meets in them, mostly one, both steps in one kernel; the
 //    shared projection is a library GEMM that adds to the result;
 //  - up to 512 rows in any order (decode): the workgroup of row i counts the earlier
@@ -27,7 +27,7 @@ typedef float ad_f32x4 __attribute__((ext_vector_type(4)));
 
 template <class T>
 struct Frag {
-  typedef T type __attribute__((ext_vector_type(8)));
+  typedef T type __attribute__((ext_vector_type(8), aligned(16)));
   typedef T loose __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 };
 
@@ -381,9 +381,10 @@ __device__ __forceinline__ float factor(const Adapters<T>& a, int id) {
 
 // ---- runs of rows ---------------------------------------------------------------
 // y = bias + c B (A x) of 16 MT neighbouring rows a workgroup of eight waves, adapter
-// by adapter (every row's products are formed, the adapter's own rows are kept): s by 16 NT of the rank into LDS, then all columns, 64 a wave in
-// turn.  Two workgroups share the adapters of the rows where a run ends in them
-// (the second has nothing to do elsewhere).
+// by adapter (every row's products are formed, the adapter's own rows are kept):
+// s by 16 NT of the rank into LDS, then all columns, 64 a wave in turn.  Two
+// workgroups share the adapters of the rows where a run ends in them (the second
+// has nothing to do elsewhere).
 constexpr int kMaxRank = 256;
 constexpr int kRunTurns = 2;
 
@@ -690,8 +691,7 @@ static bool even_call(const kda_adapter_args& d) {
   const void* ptrs[] = {d.x, d.a, d.b, d.y, d.bias};
   uintptr_t bits = 0;
   for (const void* p : ptrs) bits |= reinterpret_cast<uintptr_t>(p);
-  const int vector = d.dtype == KDA_DTYPE_F32 ? 32 : 16;
-  return d.d_in % kSlice64 == 0 && d.d_out % 64 == 0 && d.rank % 8 == 0 && bits % vector == 0;
+  return d.d_in % kSlice64 == 0 && d.d_out % 64 == 0 && d.rank % 8 == 0 && bits % 16 == 0;
 }
 
 // Workgroups along the columns: about a thousand in all, whose rows are found once.
