@@ -406,8 +406,8 @@ def unpack_states(packed: Sequence[PackedKDAState], slots: torch.Tensor | None =
     device = _one_device([t for part in parts for t in part])
     slots = _slots_arg(slots, device)
     entries = parts[0][0].shape[0]
-    if any(part[0].shape[0] != entries for part in parts):
-        raise ValueError("all layers of a pool must share the number of slots")
+    if any(t.shape[0] != entries for part in parts for t in part):
+        raise ValueError("all tensors of a pool must share the number of slots")
     n = entries if slots is None else slots.shape[0]
     _check_entries(n, entries)
     with _prep.on_device(device):

@@ -166,6 +166,31 @@ def test_slots_out_of_range_raise_and_write_nothing():
         cache.unpack_states(cache.pack_states(none), torch.tensor([0], device=DEV))
 
 
+def test_pool_tensors_that_do_not_fit_are_refused():
+    states = _caches(2, 3, 2, 16, 8)
+    pool = cache.packed_pool(states, 4)
+    slots = torch.tensor([0, 1, 2], device=DEV)
+    pool[1].v_conv_state.buffer = pool[1].v_conv_state.buffer[:3]
+    with pytest.raises(ValueError):
+        cache.unpack_states(pool, slots)
+    with pytest.raises(ValueError):
+        cache.pack_states(states, out=pool, slots=slots)
+    for other in (_caches(2, 3, 2, 16, 4), _caches(2, 3, 1, 16, 8), _caches(2, 3, 2, 16, 8, conv_dtype=torch.float16)):
+        with pytest.raises(ValueError):
+            cache.pack_states(other, out=cache.packed_pool(states, 4), slots=slots)
+    mixed = [_caches(1, 3, 2, 16, 8)[0], _caches(1, 3, 2, 16, 8, dtype=torch.bfloat16)[0]]
+    with pytest.raises(TypeError):
+        cache.pack_states(mixed)
+    with pytest.raises(ValueError):
+        cache.pack_states([_caches(1, 3, 2, 16, 8)[0], _caches(1, 2, 2, 16, 8)[0]])
+    leaf = _caches(1, 3, 2, 16, 8)[0]
+    leaf.q_conv_state.buffer.requires_grad_()
+    with pytest.raises(RuntimeError):
+        cache.pack_states([leaf])
+    with torch.no_grad():
+        cache.pack_states([leaf])
+
+
 def test_layouts_of_the_float_side():
     state = _state(3, 4, 24, 20).to(DEV)
     want = cache.pack_recurrent(state)
