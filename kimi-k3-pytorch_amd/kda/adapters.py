@@ -25,7 +25,7 @@ _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 MAX_RANK = 256
 
 
-@dataclass
+@dataclass(frozen=True)
 class AdapterStack:
     """N adapters of one projection: ``a [N, rank, in]``, ``b [N, out, rank]`` and
     the f32 factors ``scaling [N]`` (None: 1).  Adapters of a smaller rank are

@@ -96,7 +96,7 @@ class KDAState:
         )
 
 
-@dataclass
+@dataclass(frozen=True)
 class PackedState:
     """Recurrent states in 8 bits: ``values`` int8 ``[N,H,K,V]`` and one f32 scale a
     row, ``scales [N,H,K]``; row ``(n,h,k)`` stands for ``values * scales``."""
@@ -116,7 +116,7 @@ class PackedState:
             raise ValueError("packed values and scales must be contiguous")
 
 
-@dataclass
+@dataclass(frozen=True)
 class PackedKDAState:
     """A layer's decode caches at rest, or the slots of a pool of them: the
     fields of ``KDAState`` with the recurrent states in 8 bits."""

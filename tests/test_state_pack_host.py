@@ -38,6 +38,18 @@ def test_packed_types():
                            torch.zeros(3, dtype=torch.long))
 
 
+def test_what_a_kernel_reads_cannot_be_exchanged():
+    p = _packed()
+    with pytest.raises(AttributeError):
+        p.scales = torch.zeros(1)
+    pool = cache.packed_pool([_state()], 2)[0]
+    with pytest.raises(AttributeError):
+        pool.recurrent = p
+    stack = kda.adapters.AdapterStack(torch.zeros(2, 4, 8), torch.zeros(2, 6, 4))
+    with pytest.raises(AttributeError):
+        stack.b = torch.zeros(1, 6, 4)
+
+
 def test_pack_and_unpack_checks():
     with pytest.raises(ValueError):
         cache.pack_recurrent(torch.zeros(2, 4, 8))
