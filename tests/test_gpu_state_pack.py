@@ -191,6 +191,18 @@ def test_pool_tensors_that_do_not_fit_are_refused():
         cache.pack_states([leaf])
 
 
+def test_layers_of_different_sizes_in_one_call():
+    states = [_caches(1, 3, 2, 16, 8, seed=1)[0], _caches(1, 3, 1, 64, 128, seed=2)[0], _caches(1, 3, 3, 7, 5, seed=3)[0]]
+    pool = cache.packed_pool(states, 5)
+    slots = torch.tensor([4, 0, 2], device=DEV)
+    cache.pack_states(states, out=pool, slots=slots)
+    for s, p, back in zip(states, pool, cache.unpack_states(pool, slots)):
+        want = cache.pack_recurrent(s.recurrent_state)
+        assert torch.equal(p.recurrent.values[slots], want.values)
+        assert torch.equal(back.recurrent_state, cache.unpack_recurrent(want))
+        assert all(torch.equal(a, b) for a, b in zip(_parts(back), _parts(s)))
+
+
 def test_layouts_of_the_float_side():
     state = _state(3, 4, 24, 20).to(DEV)
     want = cache.pack_recurrent(state)
