@@ -509,7 +509,10 @@ namespace kda_host {
 
 using namespace kda;
 
-static bool grid_fits(int64_t n) { return n <= 0x7fffffffLL; }
+static bool rows_fit(int64_t n) { return n <= 0x7fffffffLL; }
+
+// A launch has fewer than 2^32 threads: more rows than that are served by several.
+constexpr int64_t kLaunchThreads = int64_t(1) << 31;
 
 // The kernel for rows of `vectors` 16-byte vectors: a wave a row up to 256 of them,
 // a workgroup of 256 or 1024 threads up to 4096, wider rows (0) value by value.
@@ -556,8 +559,7 @@ static void launch_rows(const AddNorm<T>& a, RowShape r, hipStream_t s) {
 }
 
 template <class T, bool Q>
-static int run_add_norm(const AddNorm<T>& a, hipStream_t s) {
-  const RowShape r = row_shape(a.width, sizeof(T), a.rows);
+static int run_add_norm_part(const AddNorm<T>& a, RowShape r, hipStream_t s) {
   if constexpr (sizeof(T) < 8) {
     if (r.threads != 0) {
       if (whole_vectors(a.width, sizeof(T), {a.x, a.r, a.w, a.h, a.y, a.q}))
@@ -569,6 +571,26 @@ static int run_add_norm(const AddNorm<T>& a, hipStream_t s) {
   }
   hipLaunchKernelGGL((add_norm_row_kernel<T, Q>), dim3(static_cast<unsigned>(a.rows)), dim3(256), 0, s, a);
   return check_launch("add_norm");
+}
+
+template <class T, bool Q>
+static int run_add_norm(const AddNorm<T>& a, hipStream_t s) {
+  const RowShape r = row_shape(a.width, sizeof(T), a.rows);
+  const int64_t step = kLaunchThreads / (r.threads != 0 ? r.threads : 256);
+  for (int64_t r0 = 0; r0 < a.rows; r0 += step) {
+    AddNorm<T> b = a;
+    const int64_t at = r0 * a.width;
+    b.rows = a.rows - r0 < step ? a.rows - r0 : step;
+    b.x += at;
+    if (a.r != nullptr) b.r += at, b.h += at;
+    if constexpr (Q)
+      b.q += at, b.scales += r0 * (a.width / a.group);
+    else
+      b.y += at;
+    const int rc = run_add_norm_part<T, Q>(b, r, s);
+    if (rc != KDA_OK) return rc;
+  }
+  return KDA_OK;
 }
 
 template <class T>
@@ -587,7 +609,7 @@ static int add_norm_typed(const void* x, const void* r, const void* w, bool wide
 
 int launch_add_norm(const void* x, const void* r, const void* w, bool wide_w, void* h, void* y, void* q, float* scales,
                     int64_t group, int64_t rows, int64_t width, double eps, int dtype, hipStream_t s) {
-  if (!grid_fits(rows)) {
+  if (!rows_fit(rows)) {
     set_detail("add_rmsnorm: %lld rows", (long long)rows);
     return KDA_ERR_UNSUPPORTED;
   }
@@ -655,7 +677,17 @@ static int add_norm_bwd_typed(const void* h, const void* w, bool wide_w, const v
   a.part = static_cast<C*>(ws), a.chunk = p.chunk;
   if (p.chunk != 0) {  // value by value
     if (dw != nullptr) a.s = a.part + p.parts * width;
-    hipLaunchKernelGGL((add_norm_bwd_row_kernel<T>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, s, a);
+    for (int64_t r0 = 0, step = kLaunchThreads / 256; r0 < rows; r0 += step) {
+      AddNormBwd<T> b = a;
+      const int64_t at = r0 * width;
+      b.h += at, b.dy += at, b.dx += at;
+      if (b.dh != nullptr) b.dh += at;
+      if (b.s != nullptr) b.s += r0;
+      const int64_t n = rows - r0 < step ? rows - r0 : step;
+      hipLaunchKernelGGL((add_norm_bwd_row_kernel<T>), dim3(static_cast<unsigned>(n)), dim3(256), 0, s, b);
+      const int rc = check_launch("add_norm_bwd");
+      if (rc != KDA_OK) return rc;
+    }
     if (dw != nullptr)
       hipLaunchKernelGGL((add_norm_dw_kernel<T>), dim3(columns, static_cast<unsigned>(p.parts)), dim3(256), 0, s, a);
   } else if constexpr (sizeof(T) < 8) {
@@ -671,7 +703,7 @@ static int add_norm_bwd_typed(const void* h, const void* w, bool wide_w, const v
 
 int launch_add_norm_bwd(const void* h, const void* w, bool wide_w, const void* dy, const void* dh, void* dx, void* dw, int64_t rows,
                         int64_t width, double eps, int dtype, void* ws, hipStream_t s) {
-  if (!grid_fits(rows)) {
+  if (!rows_fit(rows)) {
     set_detail("add_rmsnorm_bwd: %lld rows", (long long)rows);
     return KDA_ERR_UNSUPPORTED;
   }

@@ -248,3 +248,37 @@ def test_captured_calls_replay_and_streams_are_followed():
         eq, es, ehq = fused.add_rmsnorm_quant(eh, ey, w, group_size=128)
         for a, b in ((y, ey), (h, eh), (q.float(), eq.float()), (scales, es), (hq, ehq)):
             assert torch.equal(a, b)
+
+
+# A launch has fewer than 2^32 threads: 64 or 256 of them a row here.
+@pytest.mark.parametrize("dtype,rows,width", [(torch.bfloat16, (1 << 25) + 5, 2), (torch.float64, (1 << 23) + 3, 1)])
+def test_more_rows_than_a_launch_holds(dtype, rows, width):
+    gen = torch.Generator(DEV).manual_seed(3)
+    x, r, dy = (torch.randn(rows, width, generator=gen, device=DEV, dtype=torch.float32).to(dtype) for _ in range(3))
+    w = _dev(_rand(width, dtype=dtype, seed=4, scale=0.1, mean=1.0)).requires_grad_()
+    x.requires_grad_()
+    y, h = fused.add_rmsnorm(x, r, w)
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    cut = rows - 1000
+    x2, r2, dy2 = (t.detach()[cut:].clone() for t in (x, r, dy))
+    w2 = w.detach().clone().requires_grad_()
+    x2.requires_grad_()
+    y2, h2 = fused.add_rmsnorm(x2, r2, w2)
+    dx2, = torch.autograd.grad(y2, [x2], dy2)
+    assert torch.equal(y[cut:], y2) and torch.equal(h[cut:], h2) and torch.equal(dx[cut:], dx2)
+    ref, _ = ora.add_rmsnorm(x2.detach().cpu(), r2.cpu(), w2.detach().cpu())
+    assert_within(y2.detach().cpu(), ref, rounded(ref, dtype) + ref.abs() * _units(width, dtype), "y of the last rows")
+    if dtype == torch.float64:  # the reference sums in f64 too: twice the bound of a sum over the rows
+        h = h.detach()
+        terms = dy * h * (h.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+        assert_within(dw.cpu(), terms.sum(0).cpu(), 2 * (rows / 64 + 68) * unit(dtype) * terms.abs().sum(0).cpu(), "dw")
+
+
+def test_more_rows_than_a_launch_holds_in_8_bits():
+    rows, width = (1 << 25) + 5, 4
+    gen = torch.Generator(DEV).manual_seed(5)
+    x = torch.randn(rows, width, generator=gen, device=DEV, dtype=torch.float32).to(torch.bfloat16)
+    q, scales, _ = fused.add_rmsnorm_quant(x)
+    cut = rows - 1000
+    q2, scales2, _ = fused.add_rmsnorm_quant(x[cut:].clone())
+    assert torch.equal(q[cut:].view(torch.uint8), q2.view(torch.uint8)) and torch.equal(scales[cut:], scales2)
