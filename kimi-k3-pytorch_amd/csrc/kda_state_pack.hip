@@ -22,6 +22,7 @@ constexpr int kMoveThreads = 256;
 // 146 us with 8 and 154 with 4, reading back 141 and 132 (2: 195 and 163).
 constexpr int kPackSteps = 8;
 constexpr int kMoveSteps = 4;
+constexpr int64_t kMoveTiles = 0xffffffffLL / kMoveThreads;  // a launch has fewer than 2^32 threads
 constexpr float kTinyRow = 0x1p-100f;
 
 struct Move {
@@ -251,7 +252,7 @@ __global__ __launch_bounds__(kMoveThreads) void state_move_kernel(const MoveArgs
       hi = mid - 1;
   }
   const Move& d = a.d[lo];
-  const unsigned at = static_cast<unsigned>(block - d.tile0), tiles = static_cast<unsigned>(d.tiles);  // below 2^31
+  const unsigned at = static_cast<unsigned>(block - d.tile0), tiles = static_cast<unsigned>(d.tiles);  // below 2^24
   const int64_t i = at / tiles, tile = at % tiles;
   const int64_t from = a.src_index != nullptr ? a.src_index[i] : i;
   const bool there = from >= 0 && from < a.n_src;
@@ -424,12 +425,12 @@ int launch_state_move(const kda_state_tensor* t, int count, int dtype, const int
       d.tile_rows = kMoveThreads / (lanes != 0 ? lanes : 64) * (pack ? kPackSteps : kMoveSteps);
       per = (d.rows + d.tile_rows - 1) / d.tile_rows;
     }
-    if (per > 0x7fffffffLL / n) {
+    if (per > kMoveTiles / n) {
       set_detail("state_move: tensor %d is too large for one launch", i);
       return KDA_ERR_UNSUPPORTED;
     }
     d.tiles = static_cast<int32_t>(per);
-    if (a.count == kMoveMax || tiles + per * n > 0x7fffffffLL) {
+    if (a.count == kMoveMax || tiles + per * n > kMoveTiles) {
       const int err = launch_moves(a, tiles, dtype, stream);
       if (err != KDA_OK) return err;
       a.count = 0, tiles = 0;
