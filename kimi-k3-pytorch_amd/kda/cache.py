@@ -24,6 +24,7 @@ slots of a pool (``packed_pool``), ``unpack_states`` reads slots back
 from __future__ import annotations
 
 import ctypes
+from array import array
 from collections.abc import Sequence
 
 import torch
@@ -188,10 +189,8 @@ _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 def _moves(tensors: list[tuple[int, int, int | None, int, int, int]]) -> ctypes.Array:
     """``kda_state_tensor`` records (src, dst, scales, rows, width, kind) as one array of words."""
-    words = []
-    for src, dst, scales, rows, width, kind in tensors:
-        words += (src, dst, scales or 0, rows, width, kind)
-    return (ctypes.c_int64 * len(words))(*words)
+    words = array("q", [word or 0 for record in tensors for word in record])
+    return (ctypes.c_int64 * len(words)).from_buffer(words)
 
 
 def _status(device: torch.device, index: torch.Tensor | None) -> torch.Tensor | None:
