@@ -27,7 +27,6 @@ own = False
 DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 CONV = 4  # ShortConv taps (three inputs of history)
 EPS = 1e-6
-_ROOT = str(Path(__file__).resolve().parents[1] / "kimi-k3-pytorch_amd")  # where the package lies
 TINY = 2.0 ** -100  # a group whose largest magnitude is below this counts as zeros
 
 
@@ -178,8 +177,9 @@ def prepare(case, seed):
 
 
 def _kda():
-    if _ROOT not in sys.path:
-        sys.path.insert(0, _ROOT)
+    root = str(Path(__file__).resolve().parents[1] / "kimi-k3-pytorch_amd")
+    if root not in sys.path:
+        sys.path.insert(0, root)
     import kda
 
     return kda
