@@ -598,7 +598,8 @@ int kda_recurrent_fwd_packed(const void* q, const void* k, const void* v, const 
  * Low-rank adapters of many requests beside a shared projection, f32, f16 or bf16 tensors:
  *   y_m = x_m W^T + bias + scaling_a b_a (a_a x_m),  a = ids[m / span]
  * in f32.  A row with a negative id has no adapter, one with an id >= adapters is NaN.
- *   x       : [rows, d_in];  y : [rows, d_out];  bias : [d_out] or NULL (zeros)
+ *   x       : [rows, d_in], fewer than 2^28 rows (KDA_ERR_UNSUPPORTED);  y : [rows, d_out];
+ *   bias    : [d_out] or NULL (zeros)
  *   weight  : [d_out, d_in], or NULL: y without the product x W^T
  *   a       : [adapters, rank, d_in];  b : [adapters, d_out, rank]
  *   scaling : f32 [adapters] or NULL (1)

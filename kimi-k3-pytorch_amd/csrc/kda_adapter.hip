@@ -641,6 +641,10 @@ namespace kda_host {
 
 using namespace kda;
 
+// A launch has fewer than 2^32 threads along its rows: 512 for 32 of them.
+constexpr int64_t kRowsLimit = (int64_t{1} << 32) / kThreads * 32;
+int64_t adapter_rows_limit() { return kRowsLimit; }
+
 // Few rows whose ids may lie in any order go by adapter, the rest by runs.
 static bool by_adapter(const kda_adapter_args& d) { return d.rows <= kAnyOrder && d.span < 16; }
 

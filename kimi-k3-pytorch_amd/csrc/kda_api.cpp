@@ -789,6 +789,10 @@ int kda_adapter_linear(const kda_adapter_args* args, void* stream) {
     return KDA_ERR_INVALID_ARGUMENT;
   }
   const kda_adapter_args& d = *args;
+  if (d.rows >= adapter_rows_limit()) {
+    set_detail("adapter_linear: %lld rows in one call", (long long)d.rows);
+    return KDA_ERR_UNSUPPORTED;
+  }
   if (!d.x || !d.a || !d.b || !d.ids || !d.y) {
     set_detail("adapter_linear: x, a, b, ids and y must be non-null");
     return KDA_ERR_INVALID_ARGUMENT;

@@ -185,6 +185,8 @@ int launch_recurrent_packed(const void* q, const void* k, const void* v, const v
                             int64_t V, hipStream_t stream);
 
 // Adapters of many requests beside a shared projection (csrc/kda_adapter.hip).
+int64_t adapter_rows_limit();  // a call has fewer rows
+
 bool adapter_takes_projection(const kda_adapter_args& d);
 
 size_t adapter_workspace_bytes(const kda_adapter_args& d);

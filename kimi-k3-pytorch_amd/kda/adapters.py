@@ -23,6 +23,9 @@ from . import _lib, _prep
 
 _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 MAX_RANK = 256
+# Rows and elements of x or y in one native call: a launch has fewer than 2^32
+# threads (2^28 rows), and the library's product is kept under 2^31 elements.
+PIECE_ROWS, PIECE_ELEMENTS = 1 << 27, 1 << 30
 
 
 @dataclass(frozen=True)
@@ -88,6 +91,21 @@ def _check(x, weight, bias, stack, adapter_ids) -> int:
     return lead[adapter_ids.ndim:].numel()
 
 
+def row_pieces(rows: int, span: int, most: int):
+    """``(first row, rows, first id)`` of pieces of at most ``most`` rows, each of
+    which can be taken by itself with ``span`` rows an id: it begins with an id's first
+    row, or lies inside one id's rows."""
+    first = 0
+    while first < rows:
+        if span <= most:
+            n = most // span * span
+        else:
+            n = min(most, span - first % span)
+        n = min(n, rows - first)
+        yield first, n, first // span
+        first += n
+
+
 def adapter_linear(
     x: torch.Tensor,
     weight: torch.Tensor,
@@ -111,8 +129,21 @@ def adapter_linear(
     xc, a, b, ids = x.contiguous(), stack.a.contiguous(), stack.b.contiguous(), adapter_ids.contiguous()
     bias = None if bias is None else bias.contiguous()
     scaling = None if stack.scaling is None else stack.scaling.contiguous()
-    lib = _lib.load()
-    args = _lib.AdapterArgs(xc.data_ptr(), None, a.data_ptr(), b.data_ptr(), _lib.ptr(bias), _lib.ptr(scaling),
+    most = max(1, min(PIECE_ROWS, PIECE_ELEMENTS // max(d_in, d_out)))
+    with _prep.on_device(x.device):
+        if rows <= most:
+            _rows(xc, weight, bias, a, b, scaling, ids, span, y, rows)
+        else:
+            xc, flat, ids = xc.view(rows, d_in), y.view(rows, d_out), ids.flatten()
+            for first, n, first_id in row_pieces(rows, span, most):
+                _rows(xc[first:first + n], weight, bias, a, b, scaling, ids[first_id:], span, flat[first:first + n], n)
+    return y
+
+
+def _rows(x, weight, bias, a, b, scaling, ids, span, y, rows) -> None:
+    """``y [...,out]`` of ``rows`` rows ``x [...,in]``, on checked, contiguous tensors."""
+    lib, (d_out, d_in) = _lib.load(), weight.shape
+    args = _lib.AdapterArgs(x.data_ptr(), None, a.data_ptr(), b.data_ptr(), _lib.ptr(bias), _lib.ptr(scaling),
                             ids.data_ptr(), y.data_ptr(), None, 0, rows, span, d_in, d_out, a.shape[1], a.shape[0],
                             _lib.dtype_code(x.dtype), 1 if ids.dtype == torch.int64 else 0)
     ref = ctypes.addressof(args)
@@ -120,14 +151,12 @@ def adapter_linear(
         args.weight = weight.data_ptr()
         if not lib.kda_adapter_linear_takes_weight(ref):
             args.weight = None
-    with _prep.on_device(x.device):
-        args.workspace_bytes = lib.kda_adapter_linear_workspace_bytes(ref)
-        workspace = _prep.workspace(args.workspace_bytes, x.device, "adapter_linear")
-        args.workspace = _lib.ptr(workspace)
-        _lib.check(lib.kda_adapter_linear(ref, _prep.stream(x.device)))
-        if args.weight is None:
-            y.view(rows, d_out).addmm_(xc.view(rows, d_in), weight.t())
-    return y
+    args.workspace_bytes = lib.kda_adapter_linear_workspace_bytes(ref)
+    workspace = _prep.workspace(args.workspace_bytes, x.device, "adapter_linear")
+    args.workspace = _lib.ptr(workspace)
+    _lib.check(lib.kda_adapter_linear(ref, _prep.stream(x.device)))
+    if args.weight is None:
+        y.view(rows, d_out).addmm_(x.view(rows, d_in), weight.t())
 
 
 @dataclass

@@ -7,8 +7,8 @@ import ctypes
 import pytest
 import torch
 
-from kda import _lib
-from kda.adapters import AdapterStack, KDALayerAdapters, adapter_linear
+from kda import _lib, adapters
+from kda.adapters import AdapterStack, KDALayerAdapters, adapter_linear, row_pieces
 from kda.layer import KDALayerWeights, kda_attention_forward
 from tests._inputs import layer_weights
 
@@ -102,3 +102,23 @@ def test_entry_point_rejects_bad_arguments():
         lib.kda_adapter_linear_workspace_bytes(ctypes.addressof(plain))
     d = args(rank=300)
     assert lib.kda_adapter_linear_workspace_bytes(ctypes.addressof(d)) == 0
+
+
+@pytest.mark.parametrize("rows,span,most", [(1, 1, 1), (10, 1, 3), (10, 3, 4), (10, 4, 4), (25, 7, 15), (25, 10, 4), (30, 10, 3),
+                                            (9, 100, 2), (5, 100, 100), (1 << 33, 1 << 31, 1 << 27), ((1 << 30) + 1, 6, 1 << 28)])
+def test_rows_are_taken_in_pieces_of_whole_ids_or_inside_one(rows, span, most):
+    at = 0
+    for first, n, first_id in row_pieces(rows, span, most):
+        assert first == at and 1 <= n <= most
+        for m in {0, 1, n // 2, n - 1} if n > 1 else {0}:  # the piece's own rule for row m's id
+            assert (first + m) // span == first_id + m // span
+        at += n
+    assert at == rows
+
+
+def test_a_launch_never_gets_more_rows_than_it_holds():
+    # 512 threads for 32 rows, fewer than 2^32 of them
+    lib, p = _lib.load(), 4096
+    d = _lib.AdapterArgs(p, None, p, p, None, None, p, p, p, 1 << 30, 1 << 28, 16, 8, 8, 4, 2, 2, 1)
+    assert lib.kda_adapter_linear(ctypes.addressof(d), None) == _lib.KDA_ERR_UNSUPPORTED
+    assert adapters.PIECE_ROWS < 1 << 28

@@ -129,6 +129,18 @@ def test_infinities_stay_infinities(batch, tokens, dtype):
     assert torch.equal(got[y.isinf()].sign().double(), y[y.isinf()].sign())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,tokens,most", [(7, 30, 64), (3, 100, 48), (90, 1, 40), (50, 16, 600)])
+def test_more_rows_than_a_call_takes_are_served_in_pieces(batch, tokens, most, dtype, monkeypatch):
+    # the limits of a real call are 2^27 rows: here a few, pieces of whole ids and inside one
+    x, w, bias, a, b, scaling, ids = _inputs(batch, tokens, 128, 72, 16, 5, dtype)
+    monkeypatch.setattr(adapters, "PIECE_ROWS", most)
+    _check(x, w, bias, a, b, scaling, ids, _call(x, w, bias, a, b, scaling, ids))
+    monkeypatch.setattr(adapters, "PIECE_ELEMENTS", 100)  # less than a row: one at a time
+    if batch * tokens < 100:
+        _check(x, w, bias, a, b, scaling, ids, _call(x, w, bias, a, b, scaling, ids))
+
+
 def test_layouts():
     x, w, bias, a, b, scaling, ids = _dev(*_inputs(6, 3, 96, 40, 8, 4, torch.bfloat16))
     stack = adapters.AdapterStack(a, b, scaling)
