@@ -207,9 +207,10 @@ def _move(tensors, code: int, src_index, n_src: int, dst_index, n_dst: int, n: i
                                               _lib.ptr(dst_index), n_dst, n, _lib.ptr(status), stream))
 
 
-# Bytes of f32 states that a launch waits for, so that the GPU starts while the host
-# makes the records and outputs of the layers behind (8 layers of 64 MiB: 286 us a
-# store with launches of two layers, 296 us in one, 307 us with one for each).
+# Bytes of f32 states after which a call that makes its outputs itself launches what it
+# has, so that the GPU starts while the host makes the outputs of the layers behind.
+# Into a caller's pool all layers go in one native call: only there tensors can
+# overlap, and the call refuses that before anything is written.
 LAUNCH_BYTES = 100 << 20
 
 
@@ -316,7 +317,8 @@ def pack_states(states: Sequence[KDAState], *, out: Sequence[PackedKDAState] | N
     in ``out`` (one ``PackedKDAState`` a layer) batch row i goes to slot
     ``slots[i]`` (a rank-1 ``torch.long`` tensor; None: slot i, for a pool of the
     batch's size) and the other slots stay as they are; a slot named twice takes
-    the last row.  A slot out of range raises ``IndexError`` (its row is written
+    the last row.  No tensor of the pool may overlap another one or the caches.
+    A slot out of range raises ``IndexError`` (its row is written
     nowhere; in a captured graph, which no one can ask, only that).  No
     gradient: raises for states that need one."""
     states = list(states)
@@ -347,7 +349,8 @@ def pack_states(states: Sequence[KDAState], *, out: Sequence[PackedKDAState] | N
     slots = _slots_arg(slots, device)
     if slots is not None and slots.shape[0] != batch:
         raise ValueError(f"slots must name a slot for each of {batch} batch rows, got {slots.shape[0]}")
-    if out is None:
+    given = out is not None
+    if not given:
         out = []
         for s in states:
             conv = lambda c: ShortConvState(torch.empty_like(c.buffer, memory_format=torch.contiguous_format))  # noqa: E731
@@ -383,7 +386,7 @@ def pack_states(states: Sequence[KDAState], *, out: Sequence[PackedKDAState] | N
             moves.append(_pack(src[0], out[i].recurrent))
             moves += [_bytes(a, b) for a, b in zip(src[1:], dst[1:])]
             size += src[0].numel() * 4
-            if size >= LAUNCH_BYTES or len(moves) >= 60 or i + 1 == len(layers):
+            if i + 1 == len(layers) or (not given and (size >= LAUNCH_BYTES or len(moves) >= 60)):
                 _move(moves, code, None, batch, slots, entries, batch, status, stream)
                 moves, size = [], 0
         _check_slots(status, entries)

@@ -191,6 +191,31 @@ def test_pool_tensors_that_do_not_fit_are_refused():
         cache.pack_states([leaf])
 
 
+@pytest.mark.parametrize("layers,heads", [(2, 3300), (14, 2)])
+def test_pool_tensors_named_twice_are_refused_before_anything_is_written(layers, heads):
+    # 108 MiB of states a layer, and more layers than a launch holds: the call is no single launch
+    states = _caches(layers, 2, heads, 64, 64)
+    pool = cache.packed_pool(states, 3)
+    twice = [*pool[:-1], pool[0]]
+    slots = torch.tensor([2, 0], device=DEV)
+    with pytest.raises(RuntimeError, match="overlap"):
+        cache.pack_states(states, out=twice, slots=slots)
+    offsets = [kda.PackedKDAState(p.recurrent, p.q_conv_state, p.k_conv_state, p.v_conv_state, pool[0].sequence_offset)
+               for p in pool]
+    with pytest.raises(RuntimeError, match="overlap"):
+        cache.pack_states(states, out=offsets, slots=slots)
+    with pytest.raises(RuntimeError, match="overlap"):  # a cache that lies in the pool
+        within = kda.ShortConvState(pool[-1].q_conv_state.buffer[:2])
+        cache.pack_states([kda.KDAState(s.recurrent_state, within, s.k_conv_state, s.v_conv_state, s.sequence_offset)
+                           for s in states], out=pool, slots=slots)
+    for p in pool:
+        assert not bool(p.recurrent.values.any()) and not bool(p.recurrent.scales.any())
+        assert not any(bool(t.any()) for t in _parts(p))
+    cache.pack_states(states, out=pool, slots=slots)
+    for s, back in zip(states, cache.unpack_states(pool, slots)):
+        assert all(torch.equal(a, b) for a, b in zip(_parts(s), _parts(back)))
+
+
 def test_layers_of_different_sizes_in_one_call():
     states = [_caches(1, 3, 2, 16, 8, seed=1)[0], _caches(1, 3, 1, 64, 128, seed=2)[0], _caches(1, 3, 3, 7, 5, seed=3)[0]]
     pool = cache.packed_pool(states, 5)

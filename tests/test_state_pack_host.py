@@ -122,6 +122,18 @@ def test_move_entry_point_rejects_bad_arguments():
     t = cache._moves([(a, b, None, 1, 8, 0), (c, b + 8, None, 1, 8, 0)])
     assert lib.kda_state_move(ctypes.addressof(t), 2, 0, None, 3, None, 3, 3, None, None) == bad
 
+    # of many tensors too, whatever their order and distance, and one inside another
+    for first, last in ((0, 199), (199, 0), (7, 130)):
+        records = [((i + 1) << 20, (i + 501) << 20, None, 1, 8, 0) for i in range(200)]
+        records[last] = (records[last][0], records[first][1] + 16, None, 1, 8, 0)  # writes into another's destination
+        t = cache._moves(records)
+        assert lib.kda_state_move(ctypes.addressof(t), 200, 0, None, 3, None, 3, 3, None, None) == bad
+        records[last] = ((last + 1) << 20, (first + 1) << 20, None, 1, 4, 0)  # or into another's source
+        t = cache._moves(records)
+        assert lib.kda_state_move(ctypes.addressof(t), 200, 0, None, 3, None, 3, 3, None, None) == bad
+    t = cache._moves([(a, b, None, 1, 1 << 16, 0), (c, 4 << 20, None, 1, 8, 0), (b + 300, 5 << 20, None, 1, 1, 0)])
+    assert lib.kda_state_move(ctypes.addressof(t), 3, 0, None, 3, None, 3, 3, None, None) == bad
+
     def step(values=a, scales=a, slots=None, n_slots=3, dtype=2, q=a):
         return lib.kda_recurrent_fwd_packed(q, a, a, a, a, dtype, values, scales, slots, n_slots, a, a, None, 1, None,
                                             3, 3, 2, 128, 128, None)
