@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -91,6 +92,16 @@ def longest_document(offsets: list[int] | None) -> int:
 
 def stream(device: torch.device) -> int:
     return _lib.stream_of(device)
+
+
+def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """Raises for a tensor with a forward-mode tangent: a native call reads the
+    primal alone, and its result would have lost the tangent without a word."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative; call it on tensors without a tangent")
 
 
 class _Here:

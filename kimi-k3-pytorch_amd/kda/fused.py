@@ -596,6 +596,7 @@ def _check_add_norm(x, residual, weight, eps, dtypes) -> None:
         _check_device("weight", weight, x.device)
     if not eps > 0:
         raise ValueError("eps must be > 0")
+    _prep.refuse_tangents("add_rmsnorm", x, residual, weight)
     _lib.require_gpu(x)
 
 
@@ -609,8 +610,8 @@ def add_rmsnorm(
     (``h`` is ``x`` itself without a residual) and its RMSNorm
     ``y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension, ``weight [D]``
     (of that dtype, or f32) or None.  The norm reads the sum as it is stored, rounded to the dtype.
-    Differentiable in all tensors (``kda_add_rmsnorm_bwd``; the weight gradient
-    is summed in a fixed order)."""
+    Differentiable in all tensors in reverse mode (``kda_add_rmsnorm_bwd``; the weight
+    gradient is summed in a fixed order); a forward-mode tangent is refused."""
     _check_add_norm(x, residual, weight, eps, _DTYPES)
     if _needs_grad(x, residual, weight):
         y, h = _AddRMSNorm.apply(x, residual, weight, float(eps))

@@ -35,6 +35,20 @@ def test_argument_checks(call):
         call(x, x)
 
 
+@pytest.mark.parametrize("call", [fused.add_rmsnorm, fused.add_rmsnorm_quant])
+@pytest.mark.parametrize("which", ["x", "residual", "weight"])
+def test_a_tangent_is_refused_not_lost(call, which):
+    args = {"x": torch.ones(3, 64), "residual": torch.ones(3, 64), "weight": torch.ones(64)}
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            call(**{**args, which: dual})
+        with pytest.raises(RuntimeError, match="GPU"):  # a level alone changes nothing
+            call(**args)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda t: call(**{**args, which: t})[0], (args[which],), (args[which],))
+
+
 def test_quant_argument_checks():
     with pytest.raises(TypeError):
         fused.add_rmsnorm_quant(torch.zeros(3, 64, dtype=torch.float64))
