@@ -9,7 +9,8 @@ a low-rank adapter of its own: row m of the batch is
 adapters that a server keeps loaded are held stacked (``AdapterStack``), a batch
 names one per request (a negative id: none).  ``adapter_linear`` is the
 projection with them; ``layer.kda_attention_forward`` takes the stacks of its
-projections as ``KDALayerAdapters``.  For serving: there is no backward.
+projections as ``KDALayerAdapters``.  For serving: there is no derivative, and
+tensors that need a gradient or carry a forward-mode tangent are refused.
 """
 
 from __future__ import annotations
@@ -87,6 +88,7 @@ def _check(x, weight, bias, stack, adapter_ids) -> int:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in
                                        (x, weight, bias, stack.a, stack.b, stack.scaling)):
         raise RuntimeError("adapter_linear has no backward; call it under torch.no_grad() or on detached tensors")
+    _prep.refuse_tangents("adapter_linear", x, weight, bias, stack.a, stack.b, stack.scaling)
     _lib.require_gpu(x)
     return lead[adapter_ids.ndim:].numel()
 

@@ -54,6 +54,24 @@ def test_call_checks():
         call()
 
 
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "a", "b", "scaling"])
+def test_a_tangent_is_refused_not_lost(which):
+    t = {"x": torch.ones(3, 8), "weight": torch.ones(6, 8), "bias": torch.ones(6), "a": torch.ones(2, 4, 8),
+         "b": torch.ones(2, 6, 4), "scaling": torch.ones(2)}
+
+    def call(**kw):
+        t2 = {**t, **kw}
+        return adapter_linear(t2["x"], t2["weight"], t2["bias"], AdapterStack(t2["a"], t2["b"], t2["scaling"]),
+                              torch.zeros(3, dtype=torch.long))
+
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(t[which], torch.ones_like(t[which]))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            call(**{which: dual})
+        with pytest.raises(RuntimeError, match="GPU"):  # a level alone changes nothing
+            call()
+
+
 def test_layer_checks():
     weights = layer_weights(128, 1, 128, 128, dtype=torch.float32)
     w = KDALayerWeights(**weights)
