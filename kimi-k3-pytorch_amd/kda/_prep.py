@@ -94,10 +94,15 @@ def stream(device: torch.device) -> int:
     return _lib.stream_of(device)
 
 
+def forward_mode() -> bool:
+    """Whether a forward-mode level is active: only then tensors can have tangents."""
+    return forward_ad._current_level >= 0
+
+
 def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
     """Raises for a tensor with a forward-mode tangent: a native call reads the
     primal alone, and its result would have lost the tangent without a word."""
-    if forward_ad._current_level < 0:
+    if not forward_mode():
         return
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:

@@ -254,6 +254,7 @@ def pack_recurrent(state: torch.Tensor) -> PackedState:
     _check_packable(state)
     if torch.is_grad_enabled() and state.requires_grad:
         raise RuntimeError("packing has no backward; pack a detached state or call it under torch.no_grad()")
+    _prep.refuse_tangents("pack_recurrent", state)
     _one_device([state])
     out = _empty_packed(state, state.shape[0])
     n = state.shape[0]
@@ -268,6 +269,7 @@ def unpack_recurrent(packed: PackedState, slots: torch.Tensor | None = None,
     """``values * scales`` of all entries, or of ``slots`` (a slot may be named
     more than once), as ``[B,H,K,V]`` of ``dtype``.  A slot out of range raises
     ``IndexError``; in a captured graph, which no one can ask, it reads as NaN."""
+    _prep.refuse_tangents("unpack_recurrent", packed.scales)
     device = _one_device([packed.values])
     _check_float(dtype)
     slots = _slots_arg(slots, device)
@@ -329,6 +331,8 @@ def pack_states(states: Sequence[KDAState], *, out: Sequence[PackedKDAState] | N
     if not states:
         return []
     layers = [_flatten(s) for s in states]
+    if _prep.forward_mode():
+        _prep.refuse_tangents("pack_states", *(t for layer in layers for t in layer))
     shapes = [t.shape for t in layers[0]]
     dtypes = [t.dtype for t in layers[0]]
     _check_packable(layers[0][0])
@@ -405,6 +409,8 @@ def unpack_states(packed: Sequence[PackedKDAState], slots: torch.Tensor | None =
         return []
     _check_float(dtype)
     parts = [_packed_parts(p) for p in packed]
+    if _prep.forward_mode():
+        _prep.refuse_tangents("unpack_states", *(p.recurrent.scales for p in packed), *(t for part in parts for t in part))
     device = _one_device([t for part in parts for t in part])
     slots = _slots_arg(slots, device)
     entries = parts[0][0].shape[0]

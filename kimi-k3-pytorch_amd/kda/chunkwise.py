@@ -83,6 +83,7 @@ def chunkwise_kda(
     batch, tokens, *_ = validate_core_inputs(q, k, v, g, beta, None if packed is not None else initial_state, None,
                                              num_states=num_states)
     if packed is not None:
+        _prep.refuse_tangents("chunkwise_kda from a PackedState", q, k, v, g, beta, packed.scales)
         initial_state = read_packed(packed, checked_slots(packed, state_slots, q, v,
                                                           batch if num_states is None else num_states))
     valid = checked_lengths(attention_mask, batch, tokens, q.device)

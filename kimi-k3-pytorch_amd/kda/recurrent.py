@@ -72,6 +72,7 @@ def recurrent_kda(
     if packed is not None:
         if update_state_in_place:
             raise ValueError("update_state_in_place needs a float initial_state, not a PackedState")
+        _prep.refuse_tangents("recurrent_kda from a PackedState", q, k, v, g, beta, packed.scales)
         state_slots = checked_slots(packed, state_slots, q, v, batch if num_states is None else num_states)
         direct = (accumulation_dtype(v.dtype, accumulate_state_in_fp32) == torch.float32
                   and not return_states_per_token and not _chunkwise.needs_grad(q, k, v, g, beta))

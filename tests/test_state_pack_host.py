@@ -74,6 +74,34 @@ def test_pack_and_unpack_checks():
     assert pool[0].recurrent.values.shape == (5, 2, 4, 8) and pool[0].sequence_offset.shape == (5,)
 
 
+def test_a_tangent_is_refused_not_lost():
+    fw, state = torch.autograd.forward_ad, _state()
+    conv, p = state.q_conv_state, _packed()
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        recurrent = kda.KDAState(dual(state.recurrent_state), conv, conv, conv, state.sequence_offset)
+        history = kda.KDAState(state.recurrent_state, conv, kda.ShortConvState(dual(conv.buffer)), conv,
+                               state.sequence_offset)
+        scales = kda.PackedState(p.values, dual(p.scales))
+        pool = lambda packed, c: [kda.PackedKDAState(packed, c, conv, conv, state.sequence_offset)]  # noqa: E731
+        q = torch.zeros(3, 1, 2, 4)
+        args = [q, q, torch.zeros(3, 1, 2, 8), q, torch.zeros(3, 1, 2)]
+        calls = [lambda: cache.pack_recurrent(recurrent.recurrent_state), lambda: cache.unpack_recurrent(scales),
+                 lambda: cache.pack_states([state, recurrent]), lambda: cache.pack_states([history]),
+                 lambda: cache.unpack_states(pool(scales, conv)),
+                 lambda: cache.unpack_states(pool(p, kda.ShortConvState(dual(conv.buffer))))]
+        for op in (kda.recurrent_kda, kda.chunkwise_kda):
+            calls.append(lambda op=op: op(*args, scales))
+            calls += [lambda op=op, i=i: op(*args[:i], dual(args[i]), *args[i + 1:], p) for i in range(5)]
+        for call in calls:
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        for call in (lambda: cache.pack_states([state]), lambda: cache.unpack_states(pool(p, conv)),
+                     lambda: kda.recurrent_kda(*args, p)):
+            with pytest.raises(RuntimeError, match="GPU"):  # a level alone changes nothing
+                call()
+
+
 @pytest.mark.parametrize("call", [kda.recurrent_kda, kda.chunkwise_kda])
 def test_packed_initial_state_checks(call):
     q = torch.zeros(3, 1, 2, 4)
