@@ -292,11 +292,13 @@ __device__ __forceinline__ void up_columns(const Adapters<T>& a, int id, float c
   using v8 = typename Frag<U>::type;
   constexpr int P = UpType<T>::P;
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4, mycol = c0 + 16 * g;
-  ad_f32x4 d[4][MT];
+  ad_f32x4 d[P][4][MT];
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int p = 0; p < P; ++p)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) d[t][m] = ad_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) d[p][t][m] = ad_f32x4{0.f, 0.f, 0.f, 0.f};
   if (id >= 0) {
     typename Frag<T>::type raw[4];
 #pragma unroll
@@ -317,7 +319,7 @@ __device__ __forceinline__ void up_columns(const Adapters<T>& a, int id, float c
         for (int p = 0; p < P; ++p) {
           const v8 sv = *reinterpret_cast<const v8*>(&low.s[p][16 * m + li][k + 8 * g]);
 #pragma unroll
-          for (int t = 0; t < 4; ++t) d[t][m] = mma(bv[t], sv, d[t][m]);
+          for (int t = 0; t < 4; ++t) d[p][t][m] = mma(bv[t], sv, d[p][t][m]);
         }
     }
   }
@@ -328,8 +330,13 @@ __device__ __forceinline__ void up_columns(const Adapters<T>& a, int id, float c
     const int64_t row = rows[m];
     float y[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-      y[e] = c * d[e >> 2][m][e & 3] + to_float(static_cast<T>(in.bias[e / 8][e % 8]));
+    for (int e = 0; e < 16; ++e) {
+      float bs = d[0][e >> 2][m][e & 3];
+      // of an infinity the larger part decides: times what is left of s, zero or of the
+      // other sign, it would make the sum NaN
+      if constexpr (P == 2) bs = fabsf(bs) < __builtin_inff() ? bs + d[P - 1][e >> 2][m][e & 3] : bs;
+      y[e] = c * bs + to_float(static_cast<T>(in.bias[e / 8][e % 8]));
+    }
     if constexpr (WIDE) {
       for (int u = 0; u < a.parts; ++u) {
         Frag<float>::type part[2];

@@ -130,6 +130,23 @@ def test_infinities_stay_infinities(batch, tokens, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rank", [1, 40])
+@pytest.mark.parametrize("batch,tokens", [(6, 1), (60, 1), (6, 40)])
+def test_infinities_of_an_adapter_stay_infinities(batch, tokens, rank, dtype):
+    # one infinite element of adapter 1's b and one of adapter 2's a: a single infinite term in a sum each
+    x, w, bias, a, b, scaling, _ = _inputs(batch, tokens, 64, 64, rank, 3, dtype)
+    ids = torch.arange(batch) % 3
+    b[1, 7, rank - 1] = float("inf")
+    a[2, rank - 1, 3] = float("-inf")
+    got = _call(x, w, bias, a, b, scaling, ids).cpu().reshape(-1, 64)
+    rows = ids.repeat_interleave(tokens)
+    y, _, _ = ora.adapter_linear(x.reshape(-1, 64), w, bias, a, b, scaling, rows)
+    assert bool(y[rows == 1][:, 7].isinf().all()) and bool(y[rows == 2].isinf().all())
+    assert torch.equal(got.isnan(), y.isnan()) and torch.equal(got.isinf(), y.isinf())
+    assert torch.equal(got[y.isinf()].sign().double(), y[y.isinf()].sign())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("batch,tokens,most", [(7, 30, 64), (3, 100, 48), (90, 1, 40), (50, 16, 600)])
 def test_more_rows_than_a_call_takes_are_served_in_pieces(batch, tokens, most, dtype, monkeypatch):
     # the limits of a real call are 2^27 rows: here a few, pieces of whole ids and inside one
