@@ -609,7 +609,7 @@ int kda_recurrent_fwd_packed(const void* q, const void* k, const void* v, const 
  * The library forms the product itself for few rows (up to 32 with fewer than 16 rows an id,
  * f16 or bf16, d_in a multiple of 64, x, weight and a 16-byte aligned); otherwise a call with
  * a weight returns KDA_ERR_UNSUPPORTED (kda_adapter_linear_takes_weight says so beforehand): the
- * caller leaves it out and adds the product by a GEMM with beta = 1.
+ * caller leaves it out and hands in the product of its own GEMM (kda_adapter_linear_add).
  */
 typedef struct {
   const void *x, *weight, *a, *b, *bias;
@@ -627,6 +627,12 @@ int kda_adapter_linear_takes_weight(const kda_adapter_args* args);
 size_t kda_adapter_linear_workspace_bytes(const kda_adapter_args* args);
 
 int kda_adapter_linear(const kda_adapter_args* args, void* stream);
+
+/*
+ * The same beside a product that the caller formed: product = x W^T, f32 [rows, d_out], in
+ * place of args->weight (NULL).  y is the sum in f32, rounded once.
+ */
+int kda_adapter_linear_add(const kda_adapter_args* args, const float* product, void* stream);
 
 /*
  * kda_layer_decode with low-rank adapters beside the q, k, v, gate and output projections (in

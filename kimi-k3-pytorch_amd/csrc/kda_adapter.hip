@@ -8,15 +8,16 @@
 // themselves, so a call needs no sorted batch and no plan:
 //  - runs (a prompt's tokens): a workgroup owns 16 or 32 neighbouring rows and goes through
 //    the adapters it meets in them, mostly one, both steps in one kernel; the
-//    shared projection is a library GEMM that adds to the result;
+//    shared projection is a library GEMM's f32 product, which the second step adds;
 //  - up to 512 rows in any order (decode): the workgroup of row i counts the earlier
 //    rows with row i's adapter; where their number is a multiple of 16 it owns
 //    the next 16 such rows, otherwise it has nothing to do.  A launch for each
 //    step; of up to 32 rows the projection is formed beside the first.
-// Measured, bf16: 8195 rows 2048 -> 2048 rank 16, 23 us beside a GEMM of 72 us (its
-// floor is x read and y written, 11 us; the rest is one pass's latency, 1 us for
-// the ids, 6 for A x, 1 for the sums, 7 for the columns); 200 rows 4096 -> 4096
-// rank 32 of 48 adapters, 11 + 9 us beside 21 us; one row 2048 -> 2048, 7.5 + 4.4 us.
+// Measured, bf16: 8195 rows 2048 -> 2048 rank 16, 41 us beside a GEMM of 76 us (its
+// floor is x and the product read and y written, 22 us; the GEMM's adding to a 16-bit
+// bias + c B s would need 11, but rounds that sum and loses one past f16's range);
+// 200 rows 4096 -> 4096 rank 32 of 48 adapters, 10 + 11 us beside 20 to 24 us; one
+// row 2048 -> 2048, 7.8 + 6 us.
 #include <type_traits>
 
 #include "kda_launch.h"
@@ -90,7 +91,8 @@ struct Adapters {
   T* y;         // [rows, out]
   float* s;     // [splits, rows, rank]: sums over a part of the columns each
   const T* weight;  // [out, in]
-  float* wide;  // [parts, rows, out]: x W^T, over a part of the columns each; parts 0 without
+  float* wide;  // [parts, rows, out]: x W^T, over a part of the columns each (the caller's
+                // product: one part); parts 0 without
 };
 
 constexpr int kNone = -1, kMissing = -2, kNoRow = -3;
@@ -283,9 +285,9 @@ struct UpLoads {
   }
 };
 
-// y = bias + c B s (WIDE: + x W^T) of 64 columns from c0, a wave: s of 16 MT rows in
-// LDS.  rows[m]: the lane's row of tile m, or -1.
-template <class T, bool EVEN, bool WIDE, int MT, int R, int RANK>
+// y = bias + c B s + x W^T of 64 columns from c0, a wave, rounded once: s of 16 MT rows
+// in LDS.  rows[m]: the lane's row of tile m, or -1.
+template <class T, bool EVEN, int MT, int R, int RANK>
 __device__ __forceinline__ void up_columns(const Adapters<T>& a, int id, float c, const UpLoads<T, EVEN>& in,
                                            const LowRows<T, R, RANK>& low, const int (&rows)[MT], int c0) {
   using U = typename UpType<T>::type;
@@ -337,13 +339,11 @@ __device__ __forceinline__ void up_columns(const Adapters<T>& a, int id, float c
       if constexpr (P == 2) bs = fabsf(bs) < __builtin_inff() ? bs + d[P - 1][e >> 2][m][e & 3] : bs;
       y[e] = c * bs + to_float(static_cast<T>(in.bias[e / 8][e % 8]));
     }
-    if constexpr (WIDE) {
-      for (int u = 0; u < a.parts; ++u) {
-        Frag<float>::type part[2];
-        load16<float, EVEN>(a.wide + (u * a.rows + row) * a.out, mycol, a.out, part);
+    for (int u = 0; u < a.parts; ++u) {
+      Frag<float>::type part[2];
+      load16<float, EVEN>(a.wide + (u * a.rows + row) * a.out, mycol, a.out, part);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) y[e] += part[e / 8][e % 8];
-      }
+      for (int e = 0; e < 16; ++e) y[e] += part[e / 8][e % 8];
     }
     T* out = a.y + row * a.out + mycol;
     constexpr int N = 16 / sizeof(T);
@@ -366,17 +366,17 @@ __device__ __forceinline__ void up_columns(const Adapters<T>& a, int id, float c
 
 // All columns from c0 in steps, the next ones' loads ahead of the products (two
 // sets in turn: copying one to the other would wait for it).
-template <class T, bool EVEN, bool WIDE, int MT, int R, int RANK>
+template <class T, bool EVEN, int MT, int R, int RANK>
 __device__ __forceinline__ void up_all(const Adapters<T>& a, int id, float c, UpLoads<T, EVEN>& in,
                                        const LowRows<T, R, RANK>& low, const int (&rows)[MT], int c0, int step) {
   UpLoads<T, EVEN> next;
   while (c0 < a.out) {
     next.ask(a, id, c0 + step);
-    up_columns<T, EVEN, WIDE, MT>(a, id, c, in, low, rows, c0);
+    up_columns<T, EVEN, MT>(a, id, c, in, low, rows, c0);
     c0 += step;
     if (c0 >= a.out) break;
     in.ask(a, id, c0 + step);
-    up_columns<T, EVEN, WIDE, MT>(a, id, c, next, low, rows, c0);
+    up_columns<T, EVEN, MT>(a, id, c, next, low, rows, c0);
     c0 += step;
   }
 }
@@ -387,7 +387,7 @@ __device__ __forceinline__ float factor(const Adapters<T>& a, int id) {
 }
 
 // ---- runs of rows ---------------------------------------------------------------
-// y = bias + c B (A x) of 16 MT neighbouring rows a workgroup of eight waves, adapter
+// y = x W^T + bias + c B (A x) of 16 MT neighbouring rows a workgroup of eight waves, adapter
 // by adapter (every row's products are formed, the adapter's own rows are kept):
 // s by 16 NT of the rank into LDS, then all columns, 64 a wave in turn.  Two
 // workgroups share the adapters of the rows where a run ends in them (the second
@@ -443,7 +443,7 @@ __global__ __launch_bounds__(kThreads) void adapter_run_kernel(const Adapters<T>
         __syncthreads();
       }
     }
-    up_all<T, EVEN, false, MT>(a, id, c, first, low, rows, 64 * w, 64 * kWaves);
+    up_all<T, EVEN, MT>(a, id, c, first, low, rows, 64 * w, 64 * kWaves);
     __syncthreads();  // before the next adapter's sums
   }
 }
@@ -584,7 +584,7 @@ __global__ __launch_bounds__(kThreads) void adapter_both_kernel(const AdapterSet
 
 // y of 16 rows with one id (an adapter, none, or a missing one), the workgroup's four
 // waves 64 columns each in turn.
-template <class T, bool EVEN, bool WIDE>
+template <class T, bool EVEN>
 __device__ __forceinline__ void up_body(const Adapters<T>& a, LowRows<T, 16, kMaxRank>& low, int* rowS) {
   const int id = adapter_of(a, blockIdx.x), count = gather_rows<16>(a, blockIdx.x, id, rowS);
   if (count == 0) return;
@@ -620,14 +620,14 @@ __device__ __forceinline__ void up_body(const Adapters<T>& a, LowRows<T, 16, kMa
   }
   const int li = threadIdx.x & 15;
   const int rows[1] = {li < count ? rowS[li] : -1};
-  up_all<T, EVEN, WIDE, 1>(a, id, c, first, low, rows, c0, 256 * gridDim.y);
+  up_all<T, EVEN, 1>(a, id, c, first, low, rows, c0, 256 * gridDim.y);
 }
 
 template <class T, bool EVEN>
 __global__ __launch_bounds__(256) void adapter_up_kernel(const Adapters<T> a) {
   __shared__ LowRows<T, 16, kMaxRank> low;
   __shared__ int rowS[16];
-  up_body<T, EVEN, false>(a, low, rowS);
+  up_body<T, EVEN>(a, low, rowS);
 }
 
 template <class T>
@@ -637,9 +637,9 @@ __global__ __launch_bounds__(256) void adapter_up_set_kernel(const AdapterSet<T>
   const Adapters<T>& a = set.p[blockIdx.z];
   if (256 * static_cast<int>(blockIdx.y) >= a.out) return;
   if (set.even[blockIdx.z])
-    up_body<T, true, true>(a, low, rowS);
+    up_body<T, true>(a, low, rowS);
   else
-    up_body<T, false, true>(a, low, rowS);
+    up_body<T, false>(a, low, rowS);
 }
 
 }  // namespace kda
@@ -745,20 +745,21 @@ static void launch_delta(const Adapters<T>& a, bool any_order, hipStream_t s) {
 }
 
 template <class T>
-static int run_adapter_delta(const kda_adapter_args& d, hipStream_t s) {
-  const Adapters<T> a = adapters_of<T>(d);
-  if (even_call(d))
+static int run_adapter_delta(const kda_adapter_args& d, const float* product, hipStream_t s) {
+  Adapters<T> a = adapters_of<T>(d);
+  if (product != nullptr) a.wide = const_cast<float*>(product), a.parts = 1;  // read only
+  if (even_call(d) && reinterpret_cast<uintptr_t>(product) % 16 == 0)
     launch_delta<T, true>(a, by_adapter(d), s);
   else
     launch_delta<T, false>(a, by_adapter(d), s);
   return check_launch("adapter_delta");
 }
 
-int launch_adapter_delta(const kda_adapter_args& d, hipStream_t s) {
+int launch_adapter_delta(const kda_adapter_args& d, const float* product, hipStream_t s) {
   switch (d.dtype) {
-    case KDA_DTYPE_BF16: return run_adapter_delta<bf16>(d, s);
-    case KDA_DTYPE_F16: return run_adapter_delta<f16>(d, s);
-    default: return run_adapter_delta<float>(d, s);
+    case KDA_DTYPE_BF16: return run_adapter_delta<bf16>(d, product, s);
+    case KDA_DTYPE_F16: return run_adapter_delta<f16>(d, product, s);
+    default: return run_adapter_delta<float>(d, product, s);
   }
 }
 

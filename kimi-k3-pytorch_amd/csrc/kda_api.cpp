@@ -781,7 +781,7 @@ size_t kda_adapter_linear_workspace_bytes(const kda_adapter_args* args) {
   return adapter_sizes(args) ? adapter_workspace_bytes(*args) : 0;
 }
 
-int kda_adapter_linear(const kda_adapter_args* args, void* stream) {
+static int check_adapter_linear(const kda_adapter_args* args) {
   g_detail[0] = '\0';
   if (!adapter_sizes(args)) {
     set_detail("adapter_linear: positive sizes (widths up to 2^23 - 1, adapters up to 2^24 - 1), rank up to 256, "
@@ -811,8 +811,24 @@ int kda_adapter_linear(const kda_adapter_args* args, void* stream) {
     set_detail("adapter_linear: the workspace must be 16-byte aligned");
     return KDA_ERR_INVALID_ARGUMENT;
   }
+  return KDA_OK;
+}
+
+int kda_adapter_linear(const kda_adapter_args* args, void* stream) {
+  const int rc = check_adapter_linear(args);
+  if (rc != KDA_OK) return rc;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  return d.weight ? launch_adapter_set(&d, 1, s) : launch_adapter_delta(d, s);
+  return args->weight ? launch_adapter_set(args, 1, s) : launch_adapter_delta(*args, nullptr, s);
+}
+
+int kda_adapter_linear_add(const kda_adapter_args* args, const float* product, void* stream) {
+  const int rc = check_adapter_linear(args);
+  if (rc != KDA_OK) return rc;
+  if (args->weight || !product || reinterpret_cast<uintptr_t>(product) % 4 != 0) {
+    set_detail("adapter_linear_add: a product in f32 and no weight");
+    return KDA_ERR_INVALID_ARGUMENT;
+  }
+  return launch_adapter_delta(*args, product, static_cast<hipStream_t>(stream));
 }
 
 static bool layer_adapter_sizes(const kda_layer_adapters* ad) {

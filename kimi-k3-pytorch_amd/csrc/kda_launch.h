@@ -191,7 +191,8 @@ bool adapter_takes_projection(const kda_adapter_args& d);
 
 size_t adapter_workspace_bytes(const kda_adapter_args& d);
 
-int launch_adapter_delta(const kda_adapter_args& d, hipStream_t stream);
+// `product`: x W^T in f32, or null (y without it).
+int launch_adapter_delta(const kda_adapter_args& d, const float* product, hipStream_t stream);
 
 // Projections of the same few rows (adapter_takes_projection of each), up to six, each with
 // adapters or (adapters == 0) without, in two launches.

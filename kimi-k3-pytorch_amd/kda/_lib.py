@@ -143,6 +143,7 @@ SIGNATURES = {
     "kda_adapter_linear_takes_weight": (_I, [_P]),
     "kda_adapter_linear_workspace_bytes": (_S, [_P]),
     "kda_adapter_linear": (_I, [_P, _P]),
+    "kda_adapter_linear_add": (_I, [_P, _P, _P]),
     "kda_add_rmsnorm_fwd": (_I, [_P] * 3 + [_I, _P, _P, _L, _L, ctypes.c_double, _I, _P]),
     "kda_add_rmsnorm_quant": (_I, [_P] * 3 + [_I] + [_P] * 3 + [_L, _L, _L, ctypes.c_double, _I, _P]),
     "kda_add_rmsnorm_bwd_workspace_bytes": (_S, [_L, _L, _I]),

@@ -140,3 +140,16 @@ def test_a_launch_never_gets_more_rows_than_it_holds():
     d = _lib.AdapterArgs(p, None, p, p, None, None, p, p, p, 1 << 30, 1 << 28, 16, 8, 8, 4, 2, 2, 1)
     assert lib.kda_adapter_linear(ctypes.addressof(d), None) == _lib.KDA_ERR_UNSUPPORTED
     assert adapters.PIECE_ROWS < 1 << 28
+
+
+def test_adding_to_a_product_rejects_bad_arguments():
+    lib, p, bad = _lib.load(), 4096, _lib.KDA_ERR_INVALID_ARGUMENT
+
+    def call(product=p, weight=None, rows=40, workspace=p):
+        d = _lib.AdapterArgs(p, weight, p, p, None, None, p, p, workspace, 1 << 30, rows, 1, 64, 8, 4, 2, 2, 1)
+        return lib.kda_adapter_linear_add(ctypes.addressof(d), product, None)
+
+    assert call(product=None) == bad and call(product=p + 2) == bad and call(rows=0) == bad
+    assert call(weight=p, rows=20) == bad and call(weight=p) == _lib.KDA_ERR_UNSUPPORTED
+    assert call(workspace=None) == _lib.KDA_ERR_WORKSPACE
+    assert lib.kda_adapter_linear_add(None, p, None) == bad

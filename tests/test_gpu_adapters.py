@@ -70,6 +70,34 @@ def test_adapter_linear_matches_oracle(size, dtype, plain):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [(8, 1, 128, 96, 16, 3), (40, 1, 128, 96, 16, 3), (200, 1, 320, 64, 32, 40),
+                                  (24, 5, 1001, 77, 12, 9), (3, 100, 256, 128, 16, 2), (2, 300, 96, 520, 100, 4),
+                                  (1, 2100, 72, 40, 20, 1)])
+def test_the_sum_is_rounded_once(size, dtype):
+    # half a step of the result, the f32 roundings, and for bf16 what its two parts of s leave
+    x, w, bias, a, b, scaling, ids = _inputs(*size, dtype)
+    got = _call(x, w, bias, a, b, scaling, ids)
+    d_in, rank = x.shape[-1], a.shape[1]
+    y, _, (wide, low, up) = ora.adapter_linear(x.reshape(-1, d_in), w, bias, a, b, scaling,
+                                               ids.repeat_interleave(x.shape[1]))
+    units = (d_in + 8) * (wide + low) + (rank + 8) * up
+    f32 = 2.0 ** -24 * units + (2.0 ** -17 * up if dtype == torch.bfloat16 else 0.0)
+    assert_within(got.reshape(y.shape), y, rounded(y, dtype) + f32 * (1 + 2.0 ** -7), "y")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,tokens", [(4, 1), (40, 1), (4, 40), (1, 2100)])
+def test_a_part_past_the_range_meets_a_product_that_brings_it_back(batch, tokens, dtype):
+    # c B A x = 102400 (past f16's 65504), W x = -102400: all exact in f32, the bias is left
+    x = torch.ones(batch, tokens, 64, dtype=dtype)
+    w = torch.full((72, 64), -1600.0, dtype=dtype)
+    a, b = torch.ones(1, 1, 64, dtype=dtype), torch.full((1, 72, 1), 800.0, dtype=dtype)
+    bias = (torch.arange(72) / 8).to(dtype)
+    got = _call(x, w, bias, a, b, torch.tensor([2.0]), torch.zeros(batch, dtype=torch.long))
+    assert torch.equal(got.cpu(), bias.expand(batch, tokens, 72))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("batch,tokens", [(1, 1), (20, 1), (3, 5), (2, 100), (1, 600)])
 def test_all_rows_with_one_adapter_and_with_none(batch, tokens, dtype):
     x, w, bias, a, b, scaling, ids = _inputs(batch, tokens, 256, 96, 16, 4, dtype)
