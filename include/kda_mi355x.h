@@ -528,8 +528,8 @@ int kda_add_rmsnorm_fwd(const void* x, const void* residual, const void* weight,
  * The same with y in 8 bits (f32, f16 or bf16 inputs): per group of `group` elements of a row
  * (32, 64, 128 or 256, a divisor of width, or the width itself)
  *   scale = max|y| / 448,  q = e4m3(y / scale)
- * y in f32.  A group whose largest magnitude is under 2^-100 has scale 0 and zeros; one that
- * holds a NaN has scale NaN.
+ * y, scale and quotient in f32.  A group whose largest magnitude is under 2^-100 has scale 0
+ * and zeros; one that holds a NaN has scale NaN.
  *   q : OCP e4m3 bytes [rows, width];  scales : f32 [rows, width / group]
  */
 int kda_add_rmsnorm_quant(const void* x, const void* residual, const void* weight, int weight_is_f32, void* h, void* q, float* scales,

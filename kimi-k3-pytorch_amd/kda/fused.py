@@ -689,10 +689,10 @@ def add_rmsnorm_quant(
     ``q [..., D]`` in ``torch.float8_e4m3fn``, and f32 scales of one row
     (``[..., 1]``) or of ``group_size`` (32, 64, 128 or 256, a divisor of D)
     neighbouring elements (``[..., D / group_size]``), each the group's largest
-    magnitude over 448; the quotient is rounded once, from f32.  A group whose
-    largest magnitude is under 2^-100 reads back as zeros, one with a NaN as
-    NaN.  bf16, f16 and f32 tensors, for serving: it has no gradient and
-    raises for tensors that need one."""
+    magnitude over 448; ``q`` is the f32 quotient of ``y`` and its scale, rounded to
+    e4m3.  A group whose largest magnitude is under 2^-100 reads back as zeros,
+    one with a NaN as NaN.  bf16, f16 and f32 tensors, for serving: it has no
+    gradient and raises for tensors that need one."""
     _check_add_norm(x, residual, weight, eps, (torch.bfloat16, torch.float16, torch.float32))
     width = x.shape[-1]
     if group_size is not None and (group_size not in _GROUPS or width % group_size != 0):

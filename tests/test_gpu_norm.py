@@ -282,3 +282,29 @@ def test_more_rows_than_a_launch_holds_in_8_bits():
     cut = rows - 1000
     q2, scales2, _ = fused.add_rmsnorm_quant(x[cut:].clone())
     assert torch.equal(q[cut:].view(torch.uint8), q2.view(torch.uint8)) and torch.equal(scales[cut:], scales2)
+
+
+@pytest.mark.parametrize("x_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width,group", [(256, 32), (1024, None), (4096, 128), (16896, 256), (20480, None), (33024, 64)])
+def test_quotients_next_to_ties_are_those_of_the_division(width, group, x_dtype):
+    # rows of +-1 have a mean square of 1 and, with an eps under half a step, a norm of exactly 1, so y
+    # is +-weight: each group's largest magnitude m, and values within two f32 steps of where m's
+    # quotients lie in the middle of two e4m3 values.  The definition in f32, bit for bit.
+    gen = torch.Generator().manual_seed(width)
+    n = group or width
+    groups = width // n
+    e4m3 = torch.arange(0x01, 0x7f, dtype=torch.uint8).view(torch.float8_e4m3fn).float()
+    ties = (e4m3[1:] + e4m3[:-1]) / 2
+    m = (1 + torch.rand(groups, 1, generator=gen)) * torch.exp2(torch.randint(-20, 20, (groups, 1), generator=gen).float())
+    scale = m / 448
+    pick = ties[torch.randint(0, ties.numel(), (groups, n), generator=gen)]
+    near = (pick.double() * scale.double()).float()
+    steps = torch.randint(-2, 3, (groups, n), generator=gen)
+    near = (near.view(torch.int32) + steps.int()).view(torch.float32).minimum(m)
+    near[:, n // 3] = m[:, 0]
+    w = near.flatten()
+    signs = torch.randint(0, 2, (3, width), generator=gen).float() * 2 - 1
+    want = (w.view(groups, n) / scale * signs.view(3, groups, n)).to(torch.float8_e4m3fn).view(3, width)
+    q, scales, _ = fused.add_rmsnorm_quant(signs.to(x_dtype).to(DEV), None, w.to(DEV), 2.0 ** -40, group_size=group)
+    assert torch.equal(scales.cpu(), scale.view(1, groups).expand(3, groups))
+    assert torch.equal(q.cpu().view(torch.uint8), want.view(torch.uint8))
