@@ -93,6 +93,16 @@ def _check(x, weight, bias, stack, adapter_ids) -> int:
     return lead[adapter_ids.ndim:].numel()
 
 
+def _autocast(x, weight, bias, stack):
+    """The tensors of a projection in autocast's type (scaling stays f32)."""
+    dtype = torch.get_autocast_dtype("cuda")
+
+    def cast(t):
+        return t.to(dtype) if t is not None and t.is_cuda and t.dtype in _DTYPES else t
+
+    return cast(x), cast(weight), cast(bias), AdapterStack(cast(stack.a), cast(stack.b), stack.scaling)
+
+
 def row_pieces(rows: int, span: int, most: int):
     """``(first row, rows, first id)`` of pieces of at most ``most`` rows, each of
     which can be taken by itself with ``span`` rows an id: it begins with an id's first
@@ -121,7 +131,10 @@ def adapter_linear(
     each request, ``[B]``, or of each token, ``[B,T]`` (packed documents):
     ``stack.a[id]`` and ``stack.b[id]``; a negative id has none.  The call does not
     wait for the GPU, so an id past the stack cannot raise: its rows are NaN.
-    All sums are in f32 and rounded once."""
+    All sums are in f32 and rounded once.  Under autocast the tensors are taken in its
+    type, as torch's linear takes them."""
+    if torch.is_autocast_enabled("cuda"):
+        x, weight, bias, stack = _autocast(x, weight, bias, stack)
     span = _check(x, weight, bias, stack, adapter_ids)
     d_in, (d_out, rows) = x.shape[-1], (weight.shape[0], x.shape[:-1].numel())
     y = torch.empty(*x.shape[:-1], d_out, dtype=x.dtype, device=x.device)

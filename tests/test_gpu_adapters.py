@@ -186,6 +186,49 @@ def test_more_rows_than_a_call_takes_are_served_in_pieces(batch, tokens, most, d
         _check(x, w, bias, a, b, scaling, ids, _call(x, w, bias, a, b, scaling, ids))
 
 
+@pytest.mark.parametrize("batch,tokens", [(4, 1), (50, 1), (3, 60)])
+@pytest.mark.parametrize("to", [torch.bfloat16, torch.float16])
+def test_autocast_takes_the_tensors_in_its_type(batch, tokens, to):
+    x, w, bias, a, b, scaling, ids = _dev(*_inputs(batch, tokens, 64, 72, 8, 3, torch.float32))
+    cast = lambda *ts: [t.to(to) for t in ts]  # noqa: E731
+    xc, wc, bc, ac, bbc = cast(x, w, bias, a, b)
+    want = adapters.adapter_linear(xc, wc, bc, adapters.AdapterStack(ac, bbc, scaling), ids)
+    stack = adapters.AdapterStack(a, b, scaling)
+    with torch.autocast("cuda", dtype=to):
+        assert torch.nn.functional.linear(x, w, bias).dtype == to
+        assert torch.equal(adapters.adapter_linear(x, w, bias, stack, ids), want)
+        assert torch.equal(adapters.adapter_linear(xc, w, bc, stack, ids), want)
+        with pytest.raises(RuntimeError, match="backward"):
+            adapters.adapter_linear(x, w.clone().requires_grad_(), bias, stack, ids)
+        with torch.autocast("cuda", enabled=False):
+            full = adapters.adapter_linear(x, w, bias, stack, ids)
+            assert full.dtype == torch.float32
+            with pytest.raises(TypeError):
+                adapters.adapter_linear(xc, w, bias, stack, ids)
+    assert torch.equal(full, adapters.adapter_linear(x, w, bias, stack, ids))
+
+
+@pytest.mark.parametrize("mode,tokens", [("chunkwise", 40), ("decode", 1)])
+def test_a_layer_with_f32_projections_under_autocast(mode, tokens):
+    d_model, H, K = 256, 2, 128
+    weights = layer_weights(d_model, H, K, K, dtype=torch.bfloat16, biases=True, std=0.06)
+    weights = {n: t.to(DEV) if isinstance(t, torch.Tensor) else t for n, t in weights.items()}
+    names = ("q_proj", "k_proj", "v_proj", "gate_proj", "output_proj")
+    gen = torch.Generator().manual_seed(8)
+    rnd = lambda *s, std: (torch.randn(*s, generator=gen) * std).to(torch.bfloat16).to(DEV)  # noqa: E731
+    stacks = {n: adapters.AdapterStack(rnd(3, 8, d_model, std=0.06), rnd(3, d_model, 8, std=0.1)) for n in names}
+    wide = {n: adapters.AdapterStack(s.a.float(), s.b.float()) for n, s in stacks.items()}
+    x, ids = rnd(4, tokens, d_model, std=1.0), torch.tensor([2, -1, 0, 1], device=DEV)
+    lora = kda.adapters.KDALayerAdapters
+    mask = torch.ones(4, tokens, dtype=torch.bool, device=DEV)  # the composed stages
+    with torch.no_grad():
+        want = kda_attention_forward(KDALayerWeights(**weights), x, mask, None, mode, adapters=lora(**stacks), adapter_ids=ids)
+        w32 = KDALayerWeights(**{**weights, **{n: weights[n].float() for n in names}})
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            got = kda_attention_forward(w32, x.float(), mask, None, mode, adapters=lora(**wide), adapter_ids=ids)
+    assert got.hidden_states.dtype == torch.bfloat16 and torch.equal(got.hidden_states, want.hidden_states)
+
+
 def test_layouts():
     x, w, bias, a, b, scaling, ids = _dev(*_inputs(6, 3, 96, 40, 8, 4, torch.bfloat16))
     stack = adapters.AdapterStack(a, b, scaling)
