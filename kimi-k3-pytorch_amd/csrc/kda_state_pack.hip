@@ -424,7 +424,7 @@ int launch_state_move(const kda_state_tensor* t, int count, int dtype, const int
       int shift = 0;
       while (!(all >> shift & 1)) ++shift;
       d.rows = 1, d.lanes = static_cast<int16_t>(shift), d.width = static_cast<int32_t>(t[i].width >> shift);
-      per = (d.width + kMoveThreads * kMoveSteps - 1) / (kMoveThreads * kMoveSteps);
+      per = (int64_t{d.width} + kMoveThreads * kMoveSteps - 1) / (kMoveThreads * kMoveSteps);
     } else {
       d.rows = t[i].rows, d.width = static_cast<int32_t>(t[i].width);
       const bool pack = t[i].kind == KDA_MOVE_PACK;

@@ -7,8 +7,10 @@ import ctypes
 import pytest
 import torch
 
-from kda import _lib, adapters
-from kda.adapters import AdapterStack, KDALayerAdapters, adapter_linear, row_pieces
+from kda import _lib
+from kda import adapters
+from kda.adapters import AdapterStack, KDALayerAdapters, adapter_linear
+from kda.adapters import row_pieces
 from kda.layer import KDALayerWeights, kda_attention_forward
 from tests._inputs import layer_weights
 

@@ -150,7 +150,19 @@ def test_move_entry_point_rejects_bad_arguments():
     t = cache._moves([(a, b, None, 1, 8, 0), (c, b + 8, None, 1, 8, 0)])
     assert lib.kda_state_move(ctypes.addressof(t), 2, 0, None, 3, None, 3, 3, None, None) == bad
 
-    # of many tensors too, whatever their order and distance, and one inside another
+    def step(values=a, scales=a, slots=None, n_slots=3, dtype=2, q=a):
+        return lib.kda_recurrent_fwd_packed(q, a, a, a, a, dtype, values, scales, slots, n_slots, a, a, None, 1, None,
+                                            3, 3, 2, 128, 128, None)
+
+    for kw in (dict(values=None), dict(scales=None), dict(n_slots=2), dict(n_slots=0, slots=a), dict(dtype=3),
+               dict(q=None)):
+        assert step(**kw) == bad, kw
+
+
+def test_overlaps_are_refused_among_many_tensors():
+    # whatever their order and distance, and one inside another; stand-in addresses, never dereferenced
+    lib, bad = _lib.load(), _lib.KDA_ERR_INVALID_ARGUMENT
+    a, b, c = 1 << 20, 2 << 20, 3 << 20
     for first, last in ((0, 199), (199, 0), (7, 130)):
         records = [((i + 1) << 20, (i + 501) << 20, None, 1, 8, 0) for i in range(200)]
         records[last] = (records[last][0], records[first][1] + 16, None, 1, 8, 0)  # writes into another's destination
@@ -162,10 +174,9 @@ def test_move_entry_point_rejects_bad_arguments():
     t = cache._moves([(a, b, None, 1, 1 << 16, 0), (c, 4 << 20, None, 1, 8, 0), (b + 300, 5 << 20, None, 1, 1, 0)])
     assert lib.kda_state_move(ctypes.addressof(t), 3, 0, None, 3, None, 3, 3, None, None) == bad
 
-    def step(values=a, scales=a, slots=None, n_slots=3, dtype=2, q=a):
-        return lib.kda_recurrent_fwd_packed(q, a, a, a, a, dtype, values, scales, slots, n_slots, a, a, None, 1, None,
-                                            3, 3, 2, 128, 128, None)
 
-    for kw in (dict(values=None), dict(scales=None), dict(n_slots=2), dict(n_slots=0, slots=a), dict(dtype=3),
-               dict(q=None)):
-        assert step(**kw) == bad, kw
+def test_tiles_of_an_entry_are_counted_past_32_bits():
+    # an entry of nearly 2 GiB of bytes; nine of them are more tiles than a launch holds
+    t = cache._moves([(1 << 40, 1 << 44, None, 1, (1 << 31) - 1, _lib.MOVE_BYTES)])
+    assert _lib.load().kda_state_move(ctypes.addressof(t), 1, 0, None, 9, None, 9, 9, None, None) == \
+        _lib.KDA_ERR_UNSUPPORTED
