@@ -538,7 +538,8 @@ int kda_add_rmsnorm_quant(const void* x, const void* residual, const void* weigh
 /*
  * Backward of kda_add_rmsnorm_fwd: from h (x without a residual) and the gradients d_y and d_h
  * (or NULL) of its outputs, dx (the gradient of x and of the residual alike) and d_weight
- * [width] in the weight's dtype (or NULL), summed in f32 (f64) in a fixed order.
+ * [width] in the weight's dtype (or NULL), summed in f32 (f64) in a fixed order (of fewer than
+ * 2^28 columns: KDA_ERR_UNSUPPORTED).
  * Workspace: kda_add_rmsnorm_bwd_workspace_bytes(rows, width, dtype), needed with d_weight.
  */
 size_t kda_add_rmsnorm_bwd_workspace_bytes(int64_t rows, int64_t width, int dtype);

@@ -519,6 +519,9 @@ static bool rows_fit(int64_t n) { return n <= 0x7fffffffLL; }
 // A launch has fewer than 2^32 threads: more rows than that are served by several.
 constexpr int64_t kLaunchThreads = int64_t(1) << 31;
 
+// The weight gradient's sum has 1024 threads for 64 columns, in one launch.
+constexpr int64_t kDwWidth = (int64_t(1) << 32) / 1024 * 64;
+
 // The kernel for rows of `vectors` 16-byte vectors: a wave a row up to 256 of them,
 // a workgroup of 256 or 1024 threads up to 4096, wider rows (0) value by value.
 // With few rows the wave's four vectors go to four waves: latency.
@@ -710,6 +713,10 @@ int launch_add_norm_bwd(const void* h, const void* w, bool wide_w, const void* d
                         int64_t width, double eps, int dtype, void* ws, hipStream_t s) {
   if (!rows_fit(rows)) {
     set_detail("add_rmsnorm_bwd: %lld rows", (long long)rows);
+    return KDA_ERR_UNSUPPORTED;
+  }
+  if (dw != nullptr && width >= kDwWidth) {
+    set_detail("add_rmsnorm_bwd: the weight gradient of %lld columns", (long long)width);
     return KDA_ERR_UNSUPPORTED;
   }
   switch (dtype) {

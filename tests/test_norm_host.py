@@ -83,3 +83,10 @@ def test_entry_points_reject_bad_arguments():
 
     assert bwd(ws=None) == _lib.KDA_ERR_WORKSPACE and bwd(nbytes=need - 1) == _lib.KDA_ERR_WORKSPACE
     assert bwd(ws=a + 4) == bad and bwd(dy=None) == bad
+
+
+def test_a_weight_gradient_wider_than_its_launch_is_refused():
+    # 1024 threads for 64 columns, fewer than 2^32 in a launch
+    lib, a, width = _lib.load(), 4096, 1 << 28
+    need = lib.kda_add_rmsnorm_bwd_workspace_bytes(1, width, 2)
+    assert lib.kda_add_rmsnorm_bwd(a, a, 0, a, None, a, a, 1, width, 1e-6, 2, a, need, None) == _lib.KDA_ERR_UNSUPPORTED
