@@ -1,5 +1,5 @@
 // The state cache in 8 bits: decode caches written into slots of a pool and
-// read back, every tensor of every layer in one launch.
+// read back, up to 64 tensors of any layers in one launch.
 //
 // A state row (entry, head, key channel) of V values has a scale of its own:
 // the decay multiplies whole rows, so the rows of slow and fast channels differ
