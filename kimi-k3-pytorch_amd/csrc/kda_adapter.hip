@@ -715,8 +715,8 @@ template <class T, bool EVEN>
 static void launch_delta(const Adapters<T>& a, bool any_order, hipStream_t s) {
   if (!any_order) {
     // 16 rows a workgroup while 32 would leave CUs empty (2048 -> 2048 rank 16, the whole
-    // call on inputs from HBM: 2000 rows 40.6 us against 41.6, 4096 57.9 against 51.8,
-    // 8195 105 against 98)
+    // call on inputs from HBM: 2000 rows 42 us against 49 with 32, 4096 rows 70 against 63,
+    // 8195 rows 121 against 124)
     auto go = [&](auto kernel, int rows) {
       const dim3 grid(static_cast<unsigned>((a.rows + rows - 1) / rows), kRunTurns);
       hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, a);

@@ -4,8 +4,8 @@
 // over rows of `width` elements; the norm reads the stored (rounded) sum, so
 // the backward, which has h alone, differentiates the function that ran.  With
 // 8-bit output, over each group of a row (or the row):
-//   scale = max|y| / 448,  q = e4m3(y / scale), of the f32 quotient   (448: e4m3's
-// largest value)
+//   scale = max|y| / 448,  q = e4m3(y / scale)   (448: e4m3's largest value; y, scale
+//                                                 and quotient in f32)
 // and a group whose largest magnitude is under 2^-100 has scale 0 and zeros:
 // its quotients would leave f32.
 // Backward, with the gradients dy and dh of the two outputs:
@@ -72,7 +72,8 @@ __device__ __forceinline__ float group_scale(float m) { return m < kTinyGroup ? 
 __device__ __forceinline__ float scaled(float y, float scale) { return scale == 0.f ? 0.f : y / scale; }
 
 // Any width, one workgroup a row, the sum kept in h (in x without a residual)
-// between the passes: each thread reads back what it wrote itself.
+// between the passes.  Where a row has several groups, a wave reads back sums that
+// other waves wrote: the barriers in block_sum order them.
 template <class T, bool Q>
 __global__ __launch_bounds__(256) void add_norm_row_kernel(const AddNorm<T> a) {
   using C = typename NormCompute<T>::type;
@@ -122,7 +123,8 @@ __global__ __launch_bounds__(256) void add_norm_row_kernel(const AddNorm<T> a) {
 
 // Bound: the rows' bytes, each read and written once.  8192 x 7168 bf16 (470 MB)
 // 79 us, 5.9 TB/s; with e4m3 output 8192 x 4096 (236 MB) 41.4 us, 5.7 TB/s (39 with a
-// product by 448 / m in place of the division); one workgroup a row through memory (add_norm_row_kernel) took 169 us for the latter.
+// product by 448 / m in place of the division); one workgroup a row through memory
+// (add_norm_row_kernel) took 169 us for the latter.
 // Rows in registers: TPR threads a row (a wave with four rows a workgroup, or the
 // workgroup), NV vectors of 16 bytes a thread, every load of the row in flight
 // before the sum, one pass over memory.  FULL: widths of whole vectors at aligned

@@ -11,7 +11,7 @@
 // other tensors of a cache (ShortConv histories, offsets) move as bytes.
 //
 // Bound: five bytes a value.  8 layers of 32 sequences and 32 heads, 128 x 128
-// (713 MB): packed in 131 us (5.4 TB/s), read back in 131 us.
+// (713 MB): packed in one launch of 125 us (5.7 TB/s), read back in four of 37 us.
 #include <algorithm>
 #include <memory>
 #include <new>
@@ -23,7 +23,8 @@ namespace kda {
 constexpr int kMoveMax = 64;  // tensors per launch
 constexpr int kMoveThreads = 256;
 // Loads of a thread in flight.  8 layers x 32 sequences x 32 heads, 128 x 128: packing
-// 146 us with 8 and 154 with 4, reading back 141 and 132 (2: 195 and 163).
+// 125 us with 8, 130 with 4, 152 with 2; reading two of them back 38 us with 8, 37 with 4,
+// 43 with 2.
 constexpr int kPackSteps = 8;
 constexpr int kMoveSteps = 4;
 constexpr int64_t kMoveTiles = 0xffffffffLL / kMoveThreads;  // a launch has fewer than 2^32 threads
@@ -79,8 +80,7 @@ __device__ __forceinline__ RowScale row_scale(unsigned bits) {
 // Four quotients as bytes, zeros for rows without a scale.  x inv + 1.5 2^23 holds the
 // nearest whole number n in its low bits; x inv is off by 127 2^-23 at most, so n is
 // the exact quotient's unless x inv lies within 2e-5 of a tie, where the residual
-// decides.  (Deciding so for every value takes 14 instructions each, which bound
-// the kernel: 154 us against the 127 that its bytes take at the copy's rate.)
+// decides.  (Deciding so for every value, 14 instructions each: 133 us against 125.)
 __device__ __forceinline__ unsigned packed_four(const float (&x)[4], const RowScale& r) {
   constexpr float kWhole = 12582912.f;
   float n[4];
