@@ -9,10 +9,13 @@ scaling, bias and joins.
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
 import kda
+from kda import _lib
 from kda import adapters, cache, fused
 from kda.layer import KDALayerWeights, kda_attention_forward
 from oracle import kda_oracle as ora
@@ -83,6 +86,26 @@ def test_the_sum_is_rounded_once(size, dtype):
     units = (d_in + 8) * (wide + low) + (rank + 8) * up
     f32 = 2.0 ** -24 * units + (2.0 ** -17 * up if dtype == torch.bfloat16 else 0.0)
     assert_within(got.reshape(y.shape), y, rounded(y, dtype) + f32 * (1 + 2.0 ** -7), "y")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,tokens", [(9, 1), (70, 1), (3, 60)])
+def test_the_entry_point_without_a_product(batch, tokens, dtype):
+    # the C entry with neither weight nor product: bias + c B A x alone
+    x, w, bias, a, b, scaling, ids = _inputs(batch, tokens, 128, 72, 12, 4, dtype)
+    xd, bd, ad, bbd, sd, idd = _dev(x, bias, a, b, scaling, ids)
+    rows, y = batch * tokens, torch.full((batch * tokens, 72), 7.0, dtype=dtype, device=DEV)
+    lib = _lib.load()
+    args = _lib.AdapterArgs(xd.data_ptr(), None, ad.data_ptr(), bbd.data_ptr(), bd.data_ptr(), sd.data_ptr(),
+                            idd.data_ptr(), y.data_ptr(), None, 0, rows, tokens, 128, 72, 12, 4, _lib.dtype_code(dtype), 1)
+    ref = ctypes.addressof(args)
+    args.workspace_bytes = lib.kda_adapter_linear_workspace_bytes(ref)
+    workspace = torch.empty(max(1, args.workspace_bytes), dtype=torch.uint8, device=DEV)
+    args.workspace = workspace.data_ptr()
+    _lib.check(lib.kda_adapter_linear(ref, _lib.stream_of(y.device)))
+    _, delta, (_, low, up) = ora.adapter_linear(x.reshape(rows, -1), w, bias, a, b, scaling, ids.repeat_interleave(tokens))
+    f32 = 2.0 ** -24 * ((128 + 8) * low + (12 + 8) * up) + (2.0 ** -17 * up if dtype == torch.bfloat16 else 0.0)
+    assert_within(y, delta, rounded(delta, dtype) + f32 * (1 + 2.0 ** -7), "y")
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
