@@ -25,8 +25,8 @@ from . import _lib, _prep
 _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 MAX_RANK = 256
 # Rows and elements of x or y in one native call: a launch has fewer than 2^32
-# threads (2^28 rows), and the library's product is kept under 2^31 elements.
-PIECE_ROWS, PIECE_ELEMENTS = 1 << 27, 1 << 30
+# threads (2^28 rows), and the library's f32 product takes 2 GiB at most.
+PIECE_ROWS, PIECE_ELEMENTS = 1 << 27, 1 << 29
 
 
 @dataclass(frozen=True)

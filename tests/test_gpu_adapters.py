@@ -252,6 +252,21 @@ def test_a_layer_with_f32_projections_under_autocast(mode, tokens):
     assert got.hidden_states.dtype == torch.bfloat16 and torch.equal(got.hidden_states, want.hidden_states)
 
 
+@pytest.mark.parametrize("span", [8, 1 << 20])
+def test_a_batch_past_one_piece(span):
+    # 2^21 rows of 256 columns are a piece's 2^29 elements; rows on both sides of each border, and the last
+    rows, d_in, d_out = (1 << 21) + 40, 64, 256
+    rows = -(-rows // span) * span
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    rnd = lambda *s, std=1.0: (torch.randn(*s, generator=gen, device=DEV) * std).to(torch.bfloat16)  # noqa: E731
+    x, w, a, b = rnd(rows // span, span, d_in), rnd(d_out, d_in, std=0.1), rnd(5, 8, d_in, std=0.1), rnd(5, d_out, 8, std=0.3)
+    ids = torch.randint(-1, 5, (rows // span,), generator=gen, device=DEV)
+    y = adapters.adapter_linear(x, w, None, adapters.AdapterStack(a, b), ids).view(rows, d_out)
+    pick = sorted({r for edge in (0, 1 << 20, 1 << 21, rows) for r in range(max(0, edge - 40), min(rows, edge + 40))})
+    at = torch.tensor(pick, device=DEV)
+    _check(x.view(rows, d_in)[at].cpu(), w.cpu(), None, a.cpu(), b.cpu(), None, ids[at // span].cpu(), y[at])
+
+
 def test_layouts():
     x, w, bias, a, b, scaling, ids = _dev(*_inputs(6, 3, 96, 40, 8, 4, torch.bfloat16))
     stack = adapters.AdapterStack(a, b, scaling)
